@@ -237,6 +237,83 @@ int mm_orthograd_adamw_dev(const mm_param_desc* descs, const int32_t* chunk_tens
                            float ortho_eps, int rescale, int do_ortho, void* workspace, size_t workspace_bytes,
                            void* stream);
 
+/* ---- paged key-value cache -------------------------------------------------------------------
+ * No counterpart in the reference (it keeps no cache, train_autoregressive.py:97-101): the cache of rows whose lengths
+ * differ and grow past what a dense [B][H][Smax][d] array can hold, with KV heads that several query heads may share.
+ *   kpool, vpool: [n_pages][Hkv][page][d], 16-byte aligned; page a power of two in [4, 1024]; d % 4 == 0, d <= 512;
+ *   page_table:   int32 [B][width] (row stride ld_table): row b's slot s lies at place s % page of page_table[b][s / page];
+ *   weights:      float [n_pages][Hkv][page] or NULL: the attention weight each slot has drawn so far.
+ * A slot whose page number is outside [0, n_pages) or whose index is not below width * page does not exist: it is neither
+ * read nor written, and attention passes it over.  Pages that a call writes (k_new / v_new, weights, fill, evict) belong to
+ * one row alone; pages that are only read may be shared by rows (a common prompt).  Page offsets are 64-bit. */
+typedef struct {
+    const void* q;              /* [B][H][d], row stride ld_q */
+    const void* k_new;          /* [B][Hkv][d], row stride ld_k; NULL: attend from what is stored, append nothing */
+    const void* v_new;          /* [B][Hkv][d], row stride ld_v */
+    void* kpool; void* vpool;
+    void* o;                    /* [B][H][d] contiguous */
+    float* weights;             /* NULL, or: slot s gets += sum over the group's query heads of p[s]; the appended slot is set */
+    const int32_t* page_table;
+    const int32_t* lengths;     /* [B]: slots held before this token; < 0: the row sits out (o = 0, nothing stored) */
+    const int32_t* positions;   /* [B] rotary position of the token, or NULL: lengths[b] (lengths[b] - 1 without k_new); clamped to
+                                 * [0, n_pos - 1] */
+    const float* cos_t; const float* sin_t;    /* [n_pos][rot / 2]; unused at rot = 0 */
+    int64_t B, H, Hkv, d, rot, page, n_pages, width, ld_table, ld_q, ld_k, ld_v, n_pos;
+    int mode;                   /* MM_ATTN_SOFTMAX | MM_ATTN_STABLEMAX */
+    int dtype;
+    void* workspace; size_t workspace_bytes;   /* mm_paged_decode_attn_workspace(args): private to the call until it has run */
+} mm_paged_attn_args;
+/* One token of every row: q and k_new are rotated (half layout, first rot dims) at the row's position, k_new (rotated, rounded to
+ * the cache's type) and v_new are stored at slot lengths[b], and q attends over slots 0 .. lengths[b] (over 0 .. lengths[b] - 1
+ * without k_new).  lengths is not changed.  A row without a slot gets o = 0.  Scores, softmax statistics, sums and weights are
+ * float32; results do not depend on what else runs (no atomics). */
+size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* args);
+int mm_paged_decode_attn(const mm_paged_attn_args* args, void* stream);
+
+/* Runs of keys and values: token s < counts[b] of row b goes to slot start[b] + s, its key rotated at position positions[b] + s. */
+typedef struct {
+    const void* k; const void* v;               /* [B][S][Hkv][d], row strides ld_k / ld_v, batch strides bs_k / bs_v */
+    void* kpool; void* vpool;
+    float* weights;             /* NULL, or: set to 0 for the stored slots */
+    const int32_t* page_table;
+    const int32_t* start;       /* [B] or NULL: 0; < 0: nothing of the row is stored */
+    const int32_t* counts;      /* [B], used as min(counts[b], S), or NULL: S */
+    const int32_t* positions;   /* [B] or NULL: start; positions[b] + s is clamped to [0, n_pos - 1] */
+    const float* cos_t; const float* sin_t;
+    int64_t B, S, Hkv, d, rot, page, n_pages, width, ld_table, ld_k, bs_k, ld_v, bs_v, n_pos;
+    int dtype;
+} mm_paged_fill_args;
+int mm_paged_cache_fill(const mm_paged_fill_args* args, void* stream);
+
+/* Eviction by accumulated weight, per row and KV head.  A row with n = lengths[b] > budget slots keeps its newest `recent` slots and,
+ * of the n - recent older ones, the budget - recent with the greatest weight (NaN above everything, -0 = 0, ties to the lowest
+ * slot); afterwards lengths[b] = budget.  Survivors already among the first budget - recent slots stay where they are; the i-th hole
+ * there takes the i-th survivor from behind (keys carry their rotation: their order does not matter to attention), and the newest
+ * slots follow in order.  K, V and weights move together.  Rows with lengths[b] <= budget are left alone.
+ * kept: int32 [B][Hkv][budget]: the slot that slot j held before (j itself in rows left alone, -1 at or past their length). */
+size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page, int64_t width, int64_t budget, int64_t recent);
+int mm_paged_evict(void* kpool, void* vpool, float* weights, const int32_t* page_table, int32_t* lengths, int32_t* kept, int64_t B,
+                   int64_t Hkv, int64_t d, int64_t page, int64_t n_pages, int64_t width, int64_t ld_table, int64_t budget,
+                   int64_t recent, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- drafted tokens against the target's probabilities ----------------------------------------
+ * No counterpart in the reference (greedy, one token a step: train_autoregressive.py:95-110); rejection sampling whose accepted
+ * tokens are distributed as the target's own.  Draft i < n (n = counts[b] clamped to [0, K], or K) is accepted while
+ *   u[b][i] * q[b][i][x_i] < p[b][i][x_i];     a = accepted drafts;
+ * then one more token: r = max(p[b][a] - q[b][a], 0) if a < n and r has any mass, else r = p[b][a]; the smallest v with
+ * r[0] + .. + r[v] > u[b][K] * sum r, or the last v with r[v] > 0 if there is none, or 0 without any.
+ * q = NULL: the drafts have no probabilities of their own (q is 1 at x_i and 0 elsewhere).  A draft outside [0, V) is rejected.
+ * p: [B][K + 1][V], q: [B][K][V] float32 probabilities with batch and row strides; u: [B][K + 1] in [0, 1); sums and comparisons
+ * are 64-bit.  tokens: int64 [B][K + 1] = accepted drafts, the last token, then -1; accepted: int32 [B] = a. */
+typedef struct {
+    const int64_t* drafts; const float* p; const float* q; const float* u; const int32_t* counts;
+    int64_t* tokens; int32_t* accepted;
+    int64_t B, K, V, ld_drafts, bs_p, ld_p, bs_q, ld_q, ld_u;
+    void* workspace; size_t workspace_bytes;   /* mm_verify_drafts_workspace(B, V) */
+} mm_verify_args;
+size_t mm_verify_drafts_workspace(int64_t B, int64_t V);
+int mm_verify_drafts(const mm_verify_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -37,6 +37,25 @@ class GemmArgs(C.Structure):
     ]
 
 
+class PagedAttnArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("q", "k_new", "v_new", "kpool", "vpool", "o", "weights", "page_table", "lengths", "positions", "cos_t",
+                                  "sin_t")] + \
+               [(n, i64) for n in ("B", "H", "Hkv", "d", "rot", "page", "n_pages", "width", "ld_table", "ld_q", "ld_k", "ld_v", "n_pos")] + \
+               [("mode", i32), ("dtype", i32), ("workspace", vp), ("workspace_bytes", sz)]
+
+
+class PagedFillArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("k", "v", "kpool", "vpool", "weights", "page_table", "start", "counts", "positions", "cos_t", "sin_t")] + \
+               [(n, i64) for n in ("B", "S", "Hkv", "d", "rot", "page", "n_pages", "width", "ld_table", "ld_k", "bs_k", "ld_v", "bs_v",
+                                   "n_pos")] + [("dtype", i32)]
+
+
+class VerifyArgs(C.Structure):
+    _fields_ = [(n, vp) for n in ("drafts", "p", "q", "u", "counts", "tokens", "accepted")] + \
+               [(n, i64) for n in ("B", "K", "V", "ld_drafts", "bs_p", "ld_p", "bs_q", "ld_q", "ld_u")] + \
+               [("workspace", vp), ("workspace_bytes", sz)]
+
+
 _SIGNATURES = {
     "mm_version": (i32, []),
     "mm_last_error": (C.c_char_p, []),
@@ -70,6 +89,13 @@ _SIGNATURES = {
     "mm_relu2_bwd_colsum": (i32, [vp, vp, vp, vp, vp, sz, i64, i64, i32, vp]),
     "mm_cast_transpose": (i32, [vp, vp, i64, i64, i64, i32, vp]),
     "mm_cast_transpose_multi": (i32, [vp, vp, i64, vp]),
+    "mm_paged_decode_attn_workspace": (sz, [vp]),
+    "mm_paged_decode_attn": (i32, [vp, vp]),
+    "mm_paged_cache_fill": (i32, [vp, vp]),
+    "mm_paged_evict_workspace": (sz, [i64] * 6),
+    "mm_paged_evict": (i32, [vp] * 6 + [i64] * 9 + [i32, vp, sz, vp]),
+    "mm_verify_drafts_workspace": (sz, [i64, i64]),
+    "mm_verify_drafts": (i32, [vp, vp]),
     "mm_orthograd_adamw_workspace": (sz, [i64, i64]),
     "mm_orthograd_adamw": (i32, [vp, vp, vp, vp, i64, i64, i64, f32, f32, f32, f32, f32, i64, f32, i32, i32, vp, sz, vp]),
     "mm_orthograd_adamw_dev": (i32, [vp, vp, vp, vp, i64, i64, i64, vp, f32, f32, f32, f32, f32, i32, i32, vp, sz, vp]),

@@ -354,6 +354,203 @@ def decode_attn(q: Tensor, k_new: Tensor, v_new: Tensor, kcache: Tensor, vcache:
     return o
 
 
+# --------------------------------------------------------------------------- paged key-value cache
+class _OnDevice:
+    """Makes the tensors' device the current one around a launch (nothing to do where it already is)."""
+
+    def __init__(self, dev):
+        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _inference_only(who: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{who}: has no backward pass; call it under torch.no_grad()")
+
+
+def _ids(t: Optional[Tensor], name: str, B: int, dev) -> Optional[Tensor]:
+    """An int32 vector with one element per row."""
+    if t is None:
+        return None
+    _chk(t, name, torch.int32)
+    if t.shape != (B,) or t.device != dev:
+        raise RuntimeError(f"{name}: expected an int32 tensor [{B}] on {dev}, got {tuple(t.shape)} on {t.device}")
+    return t
+
+
+def _paged_geom(who: str, kpool: Tensor, vpool: Tensor, page_table: Tensor, weights: Optional[Tensor]):
+    """Checks a paged cache and returns (B, Hkv, d, page, n_pages, width)."""
+    _chk(kpool, f"{who}: kpool"); _chk(vpool, f"{who}: vpool", kpool.dtype)
+    L.dtype_code(kpool)
+    if kpool.dim() != 4 or vpool.shape != kpool.shape or vpool.device != kpool.device or vpool.data_ptr() == kpool.data_ptr():
+        raise RuntimeError(f"{who}: kpool and vpool must be two tensors [pages, KV heads, page, head_dim] on one device")
+    n_pages, Hkv, page, d = kpool.shape
+    if d % 4 or not 0 < d <= 512 or page not in (4, 8, 16, 32, 64, 128, 256, 512, 1024) or not n_pages or not Hkv:
+        raise RuntimeError(f"{who}: pages of {page} slots (a power of two, 4 to 1024), head_dim {d} (a multiple of 4, at most 512)")
+    if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.device != kpool.device \
+            or (page_table.shape[1] > 1 and page_table.stride(1) != 1) or page_table.shape[1] == 0:
+        raise RuntimeError(f"{who}: page_table must be an int32 GPU tensor [B, pages per row] with unit inner stride on the pools' device")
+    if weights is not None:
+        _chk(weights, f"{who}: weights", torch.float32)
+        if weights.shape != kpool.shape[:3] or weights.device != kpool.device:
+            raise RuntimeError(f"{who}: weights must be float32 [pages, KV heads, page] on the pools' device")
+    return page_table.shape[0], Hkv, d, page, n_pages, page_table.shape[1]
+
+
+def _rope_args(who: str, rot: int, d: int, cos_t: Optional[Tensor], sin_t: Optional[Tensor], dev) -> int:
+    """Checks the rotary tables; returns the positions they hold."""
+    if rot < 0 or rot % 2 or rot > d:
+        raise RuntimeError(f"{who}: rot={rot} must be even and at most head_dim ({d})")
+    if rot == 0:
+        return 0
+    if cos_t is None or sin_t is None:
+        raise RuntimeError(f"{who}: rot={rot} needs the cos and sin tables")
+    for t, nm in ((cos_t, "cos_t"), (sin_t, "sin_t")):
+        _f32(t, f"{who}: {nm}")
+        if t.dim() != 2 or t.shape[1] != rot // 2 or t.shape != cos_t.shape or t.shape[0] == 0 or t.device != dev:
+            raise RuntimeError(f"{who}: {nm} must be float32 [positions, {rot // 2}] on the pools' device")
+    return cos_t.shape[0]
+
+
+def _rows(t: Tensor, name: str, shape, like: Tensor) -> Tensor:
+    if not t.is_cuda or tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device \
+            or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        raise RuntimeError(f"{name}: expected {tuple(shape)} {like.dtype} with unit inner stride on {like.device}, got {tuple(t.shape)} "
+                           f"{t.dtype} on {t.device}")
+    return t
+
+
+def paged_decode_attn(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], kpool: Tensor, vpool: Tensor, page_table: Tensor,
+                      lengths: Tensor, H: int, rot: int, cos_t: Optional[Tensor], sin_t: Optional[Tensor], stablemax: bool,
+                      positions: Optional[Tensor] = None, weights: Optional[Tensor] = None) -> Tensor:
+    """decode_attn over a paged cache: one new token per row, rows of any lengths, H query heads over the pools' KV heads.
+
+    q [B, H*d], k_new / v_new [B, Hkv*d]: views with unit inner stride, un-rotated.  kpool / vpool [pages, Hkv, page, d]; page_table
+    int32 [B, pages per row]; lengths int32 [B]: slots each row holds.  k_new (rotated) and v_new are stored at slot lengths[b] and q
+    attends over slots 0 .. lengths[b]; the caller advances lengths.  k_new = v_new = None: q attends over the stored slots alone (rows
+    of drafted tokens stored by paged_cache_fill: one row per token, the table's row repeated).  positions int32 [B]: the rotary
+    position where it is not the slot (after paged_evict).  weights float32 [pages, Hkv, page]: accumulates the attention each slot
+    draws (paged_evict goes by it).  A row with lengths < 0 sits out; a row without a slot, and one that sits out, gets zeros.  A token
+    whose page the table does not hold is neither stored nor attended.  Pages written by a call belong to one row.  Returns o [B, H*d]."""
+    who = "paged_decode_attn"
+    _inference_only(who, q, k_new, v_new, kpool, vpool, weights)
+    B, Hkv, d, page, n_pages, width = _paged_geom(who, kpool, vpool, page_table, weights)
+    if H <= 0 or H % Hkv:
+        raise RuntimeError(f"{who}: {H} query heads over {Hkv} KV heads")
+    if (k_new is None) != (v_new is None):
+        raise RuntimeError(f"{who}: k_new and v_new come together")
+    _rows(q, f"{who}: q", (B, H * d), kpool)
+    if k_new is not None:
+        _rows(k_new, f"{who}: k_new", (B, Hkv * d), kpool); _rows(v_new, f"{who}: v_new", (B, Hkv * d), kpool)
+    dev = kpool.device
+    _ids(lengths, f"{who}: lengths", B, dev); _ids(positions, f"{who}: positions", B, dev)
+    o = torch.empty((B, H * d), dtype=q.dtype, device=dev)
+    a = L.PagedAttnArgs(
+        q.data_ptr(), L.ptr(k_new), L.ptr(v_new), kpool.data_ptr(), vpool.data_ptr(), o.data_ptr(), L.ptr(weights), page_table.data_ptr(),
+        lengths.data_ptr(), L.ptr(positions), L.ptr(cos_t) if rot else None, L.ptr(sin_t) if rot else None, B, H, Hkv, d, rot, page, n_pages,
+        width, page_table.stride(0), q.stride(0), 0 if k_new is None else k_new.stride(0), 0 if v_new is None else v_new.stride(0),
+        _rope_args(who, rot, d, cos_t, sin_t, dev), int(stablemax), L.dtype_code(kpool))
+    nbytes = L.lib().mm_paged_decode_attn_workspace(C.byref(a))
+    with _OnDevice(dev):
+        # a buffer of its own per call: calls on two streams, and graphs captured on one stream and replayed beside each other, share none
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        a.workspace, a.workspace_bytes = L.ptr(ws), nbytes
+        L.check(L.lib().mm_paged_decode_attn(C.byref(a), L.cur_stream()), "mm_paged_decode_attn")
+    return o
+
+
+def paged_cache_fill(k: Tensor, v: Tensor, kpool: Tensor, vpool: Tensor, page_table: Tensor, rot: int, cos_t: Optional[Tensor],
+                     sin_t: Optional[Tensor], start: Optional[Tensor] = None, counts: Optional[Tensor] = None,
+                     positions: Optional[Tensor] = None, weights: Optional[Tensor] = None) -> None:
+    """Stores runs in a paged cache: k, v [B, S, Hkv*d] (views with unit inner stride, k un-rotated).  Token s < counts[b] of row b goes to
+    slot start[b] + s (start: default 0), its key rotated at positions[b] + s (default start[b] + s).  start, counts, positions: int32
+    [B].  Rows with start < 0 store nothing; tokens whose page the table does not hold are left out; the rest of a padded batch is not
+    read.  weights: set to 0 for the stored slots."""
+    who = "paged_cache_fill"
+    _inference_only(who, k, v, kpool, vpool, weights)
+    B, Hkv, d, page, n_pages, width = _paged_geom(who, kpool, vpool, page_table, weights)
+    if k.dim() != 3:
+        raise RuntimeError(f"{who}: k must be [B, S, KV heads * head_dim]")
+    S = k.shape[1]
+    _rows(k, f"{who}: k", (B, S, Hkv * d), kpool); _rows(v, f"{who}: v", (B, S, Hkv * d), kpool)
+    dev = kpool.device
+    _ids(start, f"{who}: start", B, dev); _ids(counts, f"{who}: counts", B, dev); _ids(positions, f"{who}: positions", B, dev)
+    a = L.PagedFillArgs(
+        k.data_ptr(), v.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), L.ptr(weights), page_table.data_ptr(), L.ptr(start), L.ptr(counts),
+        L.ptr(positions), L.ptr(cos_t) if rot else None, L.ptr(sin_t) if rot else None, B, S, Hkv, d, rot, page, n_pages, width,
+        page_table.stride(0), k.stride(1), k.stride(0), v.stride(1), v.stride(0), _rope_args(who, rot, d, cos_t, sin_t, dev),
+        L.dtype_code(kpool))
+    with _OnDevice(dev):
+        L.check(L.lib().mm_paged_cache_fill(C.byref(a), L.cur_stream()), "mm_paged_cache_fill")
+
+
+def paged_evict(kpool: Tensor, vpool: Tensor, weights: Tensor, page_table: Tensor, lengths: Tensor, budget: int, recent: int) -> Tensor:
+    """Cuts every row with lengths[b] > budget down to `budget` slots, per KV head: the newest `recent` and, of the older ones, those with the
+    greatest accumulated weight (ties: the lowest slot).  Survivors among the first budget - recent slots stay where they are, the holes
+    there are filled from behind in order, the newest follow; K, V and weights move together and lengths[b] becomes budget, in place.
+    Later tokens carry their own rotary position (paged_decode_attn's positions).  Returns int32 [B, Hkv, budget]: the slot that
+    each slot held before (its own number in rows left alone, -1 past their length)."""
+    who = "paged_evict"
+    if weights is None:
+        raise RuntimeError(f"{who}: weights are what it goes by")
+    _inference_only(who, kpool, vpool, weights)
+    B, Hkv, d, page, n_pages, width = _paged_geom(who, kpool, vpool, page_table, weights)
+    if not 0 < budget < 1 << 30 or not 0 <= recent <= budget:
+        raise RuntimeError(f"{who}: budget={budget} recent={recent}: 0 <= recent <= budget and budget > 0")
+    dev = kpool.device
+    _ids(lengths, f"{who}: lengths", B, dev)
+    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
+    nbytes = L.lib().mm_paged_evict_workspace(B, Hkv, page, width, budget, recent)
+    with _OnDevice(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        L.check(L.lib().mm_paged_evict(kpool.data_ptr(), vpool.data_ptr(), weights.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
+                                       kept.data_ptr(), B, Hkv, d, page, n_pages, width, page_table.stride(0), budget, recent,
+                                       L.dtype_code(kpool), L.ptr(ws), nbytes, L.cur_stream()), "mm_paged_evict")
+    return kept
+
+
+def verify_drafts(drafts: Tensor, p: Tensor, u: Tensor, q: Optional[Tensor] = None, counts: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """Rejection sampling of drafted tokens: draft i is accepted while u[b, i] * q[b, i, x_i] < p[b, i, x_i]; one more token follows, drawn
+    with u[b, K] from max(p - q, 0) at the first rejected draft, or from p behind the last (the smallest v whose cumulative sum exceeds
+    u times the sum).  Tokens so chosen are distributed as the target's own.
+
+    drafts int64 [B, K] (K may be 0); p float32 [B, K+1, V]: the target's probabilities at each draft and behind the last; u float32
+    [B, K+1] in [0, 1); q float32 [B, K, V]: the draft's probabilities, None for drafts without any (copied ones: q is 1 at the draft);
+    counts int32 [B]: drafts a row really has.  Rows may be strided, the inner stride is 1.  Returns tokens int64 [B, K+1] (accepted
+    drafts, the last token, then -1) and the number accepted, int32 [B]."""
+    who = "verify_drafts"
+    _inference_only(who, p, q)
+    if drafts.dim() != 2 or p.dim() != 3 or not drafts.is_cuda or drafts.dtype != torch.int64 or drafts.device != p.device \
+            or (drafts.shape[1] > 1 and drafts.stride(1) != 1):
+        raise RuntimeError(f"{who}: drafts must be an int64 GPU tensor [B, K] with unit inner stride on the device of p [B, K + 1, V]")
+    B, K = drafts.shape
+    V = p.shape[2]
+    if p.dtype != torch.float32 or V == 0:
+        raise TypeError(f"{who}: p must hold float32 probabilities [B, K + 1, V], got {p.dtype} {tuple(p.shape)}")
+    _rows(p, f"{who}: p", (B, K + 1, V), p); _rows(u, f"{who}: u", (B, K + 1), p)
+    if q is not None:
+        _rows(q, f"{who}: q", (B, K, V), p)
+    dev = p.device
+    _ids(counts, f"{who}: counts", B, dev)
+    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=dev)
+    accepted = torch.empty(B, dtype=torch.int32, device=dev)
+    nbytes = L.lib().mm_verify_drafts_workspace(B, V)
+    with _OnDevice(dev):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        a = L.VerifyArgs(drafts.data_ptr(), p.data_ptr(), L.ptr(q), u.data_ptr(), L.ptr(counts), tokens.data_ptr(), accepted.data_ptr(),
+                         B, K, V, drafts.stride(0), p.stride(0), p.stride(1), 0 if q is None else q.stride(0),
+                         0 if q is None else q.stride(1), u.stride(0), L.ptr(ws), nbytes)
+        L.check(L.lib().mm_verify_drafts(C.byref(a), L.cur_stream()), "mm_verify_drafts")
+    return tokens, accepted
+
+
 # --------------------------------------------------------------------------- small pieces
 def layerscale_bwd(dout: Tensor, z: Tensor, gamma: Tensor, rowscale: Optional[Tensor], rows_per_scale: int):
     _chk(dout, "dout"); _chk(z, "z", dout.dtype)
