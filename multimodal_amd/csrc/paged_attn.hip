@@ -1,111 +1,538 @@
 // Attention of one token over a paged key-value cache, with its append, and the storing of runs (include/mmhip.h).
+//
+//   x_hs = q'_h . K_s / sqrt(d),  p = softmax_s(x) | stablemax_s(x),  o_h = sum_s p_hs V_s
+//
+// The cache is read once: 2 d values per slot and KV head against 4 d operations per query head, so HBM bounds it as long as the
+// operations are cheap.  On the vector units they are not (shared heads: 2 G operations per byte in bf16, and the unpacking on top);
+// on the matrix units a 16 x 16 tile costs the same for 1 to 16 query heads, a few per cent of the time its bytes need.  So:
+//   - the query heads of a KV head are the 16 columns of a tile, 16 slots its rows: S = K Q^T;
+//   - a lane's S values (column = its head, rows 4 g .. 4 g + 3 of each tile) are exactly the B operand of O^T = V^T P^T when
+//     the 32 slots of a step are taken in the order (tile, group, row): probabilities never leave their lane;
+//   - V comes straight from global memory too: a lane loads 16 bytes of each of "its" eight slots (a row is read whole by 16 lanes) and
+//     transposes 8 x 8 values in registers (32 v_perm per 128 columns), which is the A operand.  No LDS traffic in the loop.
+// The rotated q is kept as three bf16 terms (24 bits) and p as two (15 bits): the products are then as good as float32 ones, and what is
+// rounded is what the caller asked to be rounded (stored keys, the output).  Each term but the last is truncated, so that all have one
+// sign, and none is 0 unless the value is: an infinite key or value gives what it gives in one product (inf - inf and 0 * inf do not arise).
+// float32 runs the same walk on the f32 matrix instruction.
+// A workgroup is four waves that take 32 slots each in turn, with their own running maximum and sum, merged at the end; long caches
+// are split over workgroups and a second kernel joins them (and adds the weights up).  The token's own key and value are taken
+// from the inputs, not from the cache, so nothing waits for the append.
 #include "paged.h"
+#include <type_traits>
+
+typedef __attribute__((ext_vector_type(4))) unsigned u4_t;
+typedef __attribute__((ext_vector_type(2))) unsigned u2_t;
 
 struct PagedP {
     const void* q; const void* kn; const void* vn; void* kpool; void* vpool; void* o; float* w; const int* lengths; const int* positions;
-    const float* cos_t; const float* sin_t; float* sc; PagedMap map;
-    int B, H, Hkv, G, d, rot, n_pos; long ld_q, ld_k, ld_v; float scale;
+    const float* cos_t; const float* sin_t; PagedMap map;
+    float* part; float2* stat; float* sc;       // per (row, head, split): unscaled output [d], (max, sum); scores [row][head][capacity]
+    int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, stable; long ld_q, ld_k, ld_v; float scale;
 };
 
-__device__ __forceinline__ int paged_pos(const PagedP& p, int b) {
-    const int n = p.lengths[b];
-    const int pos = p.positions ? p.positions[b] : (p.kn ? n : n - 1);
-    return min(max(pos, 0), p.n_pos - 1);
+__device__ __forceinline__ int paged_pos(const int* positions, const int* lengths, bool append, int n_pos, int b) {
+    const int n = lengths[b];
+    const int pos = positions ? positions[b] : (append ? n : n - 1);
+    return min(max(pos, 0), n_pos - 1);
 }
-// element c of a head, rotated at table row `cs` / `sn`
+// element c of a head, rotated (half layout over the first rot dims) at the table row cs / sn
 template <typename T> __device__ __forceinline__ float rotated(const T* x, int c, int rot, const float* cs, const float* sn) {
     const int half = rot >> 1;
     const float a = to_f(x[c]);
     if (c >= rot) return a;
     const int i = c < half ? c : c - half;
     const float o = to_f(x[c < half ? c + half : c - half]);
-    return c < half ? a * cs[i] - o * sn[i] : a * cs[i] + o * sn[i];
+    return c < half ? fmaf(a, cs[i], -(o * sn[i])) : fmaf(a, cs[i], o * sn[i]);
+}
+// stablemax's s(x); the reciprocal is within one unit in the last place
+__device__ __forceinline__ float stable_s(float x) { return x < 0.f ? __builtin_amdgcn_rcpf(1.f - x + 1e-9f) : x + 1.f; }
+
+// over the four lanes that hold a head's values (lane ^ 16, lane ^ 32)
+__device__ __forceinline__ float quad_max(float v) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+__device__ __forceinline__ float quad_sum(float v) {
+    v += __shfl_xor(v, 16);
+    v += __shfl_xor(v, 32);
+    return v;
+}
+// barrier that orders LDS only: loads from global memory stay in flight across it
+__device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
-template <typename T> __global__ __launch_bounds__(64) void paged_append_k(const PagedP p) {
-    const int b = blockIdx.x, h = blockIdx.y, n = p.lengths[b];
-    if (n < 0) return;
-    const long row = p.map.row(b, h, n);
+// ------------------------------------------------------------------------------------------------ operands of one step (16 NT slots)
+// VE: columns a lane loads of a V row (16 lanes x VE = one slab), NS: slabs of a head, NT: tiles of 16 slots in a step, AL8: rows are
+// multiples of 8 values (16-byte pieces).  K of the whole step is in registers; of V up to two slabs, the others follow as those are used
+// up (a head of 512 would need 512 registers for its step otherwise).
+template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
+    static constexpr bool BF = std::is_same<T, bf16>::value;
+    static constexpr int VE = VE_, NS = NS_, NT = NT_, J = 4 * NT, DP = 16 * VE * NS;
+    static constexpr int PE = BF ? 8 : 4, CW = 4 * PE, KC = DP / CW;           // values in a lane's piece of K, columns of a matrix instruction
+    static constexpr int QT = BF ? 3 : 1, QFRAG = QT * KC * 64 * 16;           // terms of q, bytes of its fragments in LDS
+    static constexpr int VB = NS < 2 ? NS : 2;
+    static constexpr bool QREG = DP <= 128;                                    // wider heads read the q fragments from LDS every step
+    static_assert(!BF || NT == 2, "the bf16 products take 32 slots");
+    typedef typename std::conditional<VE * sizeof(T) == 16, u4_t, u2_t>::type v_t;
+    typedef __attribute__((ext_vector_type(8))) __bf16 frag_t;
+    u4_t k[NT][KC];
+    v_t v[VB][J];
+    u4_t q[QREG ? QT : 1][QREG ? KC : 1];
+
+    __device__ __forceinline__ void load_k(const T* pool, const long (&row)[NT], int d, int g) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const T* r = pool + row[t] * d;
+#pragma unroll
+            for (int c = 0; c < KC; c++) {
+                const int col = c * CW + g * PE;
+                if constexpr (AL8) {
+                    k[t][c] = *reinterpret_cast<const u4_t*>(r + (col < d ? col : 0));
+                } else {
+                    const u2_t a = *reinterpret_cast<const u2_t*>(r + (col < d ? col : 0)), b = *reinterpret_cast<const u2_t*>(r + (col + 4 < d ? col + 4 : 0));
+                    k[t][c] = u4_t{a[0], a[1], b[0], b[1]};
+                }
+            }
+        }
+    }
+    // pieces past column d become 0 (their q is 0 too, but 0 * inf is not)
+    __device__ __forceinline__ void trim_k(int d, int g) {
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+            if (c * CW + CW > d) {
+                const int col = c * CW + g * PE;
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    if (col >= d) k[t][c] = u4_t{0u, 0u, 0u, 0u};
+                    else if (!AL8 && col + 4 >= d) { k[t][c][2] = 0u; k[t][c][3] = 0u; }
+                }
+            }
+    }
+    __device__ __forceinline__ void load_slab(int s, const T* pool, const long (&row)[NT], int d, int li) {
+        const int col = (s * 16 + li) * VE, cc = col < d ? col : 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) v[s % VB][t * 4 + i] = *reinterpret_cast<const v_t*>(pool + (row[t] + i) * d + cc);
+    }
+    __device__ __forceinline__ void load_v(const T* pool, const long (&row)[NT], int d, int li) {
+#pragma unroll
+        for (int s = 0; s < VB; s++) load_slab(s, pool, row, d, li);
+    }
+    // the token's own key, from LDS, as slot 0 of the step
+    __device__ __forceinline__ void own_k(const T* ks, int li, int g) {
+#pragma unroll
+        for (int t = 0; t < NT; t++)
+#pragma unroll
+            for (int c = 0; c < KC; c++) k[t][c] = u4_t{0u, 0u, 0u, 0u};
+        if (li == 0)
+#pragma unroll
+            for (int c = 0; c < KC; c++) k[0][c] = *reinterpret_cast<const u4_t*>(ks + c * CW + g * PE);
+    }
+    // q fragments: value (head, column), in lane (group * 16 + head) of its chunk, as QT terms
+    static __device__ __forceinline__ void put_q(char* lds, int head, int c, float x) {
+        T* f = (T*)lds;
+        const int at = ((c / CW) * 64 + (c / PE % 4) * 16 + head) * PE + c % PE;
+        if constexpr (!BF) { f[at] = x; return; }
+        const float least = x == 0.f ? 0.f : copysignf(0x1p-100f, x);
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+            const float h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+            f[t * KC * 64 * PE + at] = from_f<T>(t && h == 0.f ? least : h);
+            x -= h;
+        }
+    }
+    __device__ __forceinline__ void get_q(const char* lds, int lane) {
+        if constexpr (QREG)
+#pragma unroll
+            for (int t = 0; t < QT; t++)
+#pragma unroll
+                for (int c = 0; c < KC; c++) q[t][c] = *reinterpret_cast<const u4_t*>(lds + ((t * KC + c) * 64 + lane) * 16);
+    }
+    // the scores of the step's tiles.  Columns that are not rotated are exact in q's first term.
+    __device__ __forceinline__ void scores(const char* lds, int lane, int rot, f32x4_t (&s)[NT]) const {
+#pragma unroll
+        for (int h = 0; h < NT; h++) s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < KC; c++)
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                if (t && c * CW >= rot) break;
+                u4_t qf;
+                if constexpr (QREG) qf = q[t][c];
+                else qf = *reinterpret_cast<const u4_t*>(lds + ((t * KC + c) * 64 + lane) * 16);
+#pragma unroll
+                for (int h = 0; h < NT; h++) {
+                    if constexpr (BF) {
+                        s[h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(frag_t, k[h][c]), __builtin_bit_cast(frag_t, qf), s[h], 0, 0, 0);
+                    } else {
+                        const f32x4_t kf = __builtin_bit_cast(f32x4_t, k[h][c]), qq = __builtin_bit_cast(f32x4_t, qf);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s[h], 0, 0, 0);
+                    }
+                }
+            }
+    }
+    // acc[slab][column][4] += V^T P^T over one slab; slots whose bit is not set have p = 0, and their V must not be inf or NaN
+    __device__ __forceinline__ void slab(int s, const float (&p)[J], unsigned ok, f32x4_t (&acc)[NS][VE]) {
+        v_t (&w)[J] = v[s % VB];
+        if (__ballot(ok != (1u << J) - 1)) {
+#pragma unroll
+            for (int j = 0; j < J; j++) if (!(ok >> j & 1)) w[j] = v_t{};
+        }
+        if constexpr (BF) {
+            typedef __attribute__((ext_vector_type(2))) float f2_t;
+            typedef __attribute__((ext_vector_type(2))) __bf16 b2_t;
+            unsigned hi[4], lo[4];
+#pragma unroll
+            for (int m = 0; m < 4; m++) {
+                const unsigned a = __float_as_uint(p[2 * m]), b = __float_as_uint(p[2 * m + 1]);
+                hi[m] = __builtin_amdgcn_perm(b, a, 0x07060302u);
+                lo[m] = __builtin_bit_cast(unsigned, __builtin_convertvector((f2_t{fmaxf(p[2 * m] - __uint_as_float(a & 0xffff0000u), 0x1p-100f),
+                                                                                  fmaxf(p[2 * m + 1] - __uint_as_float(b & 0xffff0000u), 0x1p-100f)}), b2_t));
+            }
+            const frag_t ph = __builtin_bit_cast(frag_t, (u4_t{hi[0], hi[1], hi[2], hi[3]})), pl = __builtin_bit_cast(frag_t, (u4_t{lo[0], lo[1], lo[2], lo[3]}));
+#pragma unroll
+            for (int e = 0; e < VE; e++) {
+                unsigned x[4];
+#pragma unroll
+                for (int m = 0; m < 4; m++)                                    // two slots' halfwords side by side
+                    x[m] = __builtin_amdgcn_perm(w[2 * m + 1][e >> 1], w[2 * m][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
+                const frag_t a = __builtin_bit_cast(frag_t, (u4_t{x[0], x[1], x[2], x[3]}));
+                acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ph, acc[s][e], 0, 0, 0);
+                acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pl, acc[s][e], 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const f32x4_t x = __builtin_bit_cast(f32x4_t, w[j]);
+#pragma unroll
+                for (int e = 0; e < VE; e++) acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], p[j], acc[s][e], 0, 0, 0);
+            }
+        }
+    }
+    __device__ __forceinline__ void gather(const float (&p)[J], unsigned ok, const T* pool, const long (&row)[NT], int d, int li, f32x4_t (&acc)[NS][VE]) {
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            slab(s, p, ok, acc);
+            if (s + VB < NS) load_slab(s + VB, pool, row, d, li);
+        }
+    }
+    // the token's own value, from LDS
+    __device__ __forceinline__ void gather_own(const float (&p)[J], const T* vs, int li, int g, f32x4_t (&acc)[NS][VE]) {
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+#pragma unroll
+            for (int j = 0; j < J; j++) v[s % VB][j] = v_t{};
+            if (g == 0) v[s % VB][0] = *reinterpret_cast<const v_t*>(vs + (s * 16 + li) * VE);
+            slab(s, p, (1u << J) - 1, acc);
+        }
+    }
+};
+
+// ------------------------------------------------------------------------------------------------ the walk
+template <typename T, int VE, int NS, int NT, bool AL8>
+__global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void paged_attn_k(const PagedP p) {
+    typedef Step<T, VE, NS, NT, AL8> S_t;
+    constexpr int SW = 16 * VE, DP = SW * NS, ST = 16 * NT, RD = 4 * ST, J = 4 * NT;      // a wave's step, a round of the four waves
+    constexpr int MERGE = 4 * 16 * SW * 4, QB = S_t::QFRAG;
+    __shared__ __attribute__((aligned(16))) char lds[QB > MERGE ? QB : MERGE];          // q fragments; at the end the waves' outputs
+    __shared__ __attribute__((aligned(16))) T own_k[DP], own_v[DP];
+    __shared__ float st_m[4][16], st_l[4][16];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, g = lane >> 4;
+    int id = blockIdx.x;
+    const int split = id % p.nsplit; id /= p.nsplit;
+    const int ct = id % p.ctiles; id /= p.ctiles;
+    const int hk = id % p.Hkv, b = id / p.Hkv;
+    const int d = p.d, cap = p.map.capacity(), len = p.lengths[b];
+    const int h0 = hk * p.G + ct * 16, nh = min(16, p.G - ct * 16);                     // this tile's query heads
+    const int n = min(max(len, 0), cap);                                                // slots in the cache
+    const int cover = len < 0 ? 0 : min(n + (p.kn ? 1 : 0), cap);
+    const int lo = split * p.chunk, hi = min(n, lo + p.chunk);
+    if (split && lo >= cover) return;
+    const bool mine = p.kn && len >= 0 && len < cap && len >= lo && len < lo + p.chunk; // the new token falls into this split
+    const long own_row = mine ? p.map.row(b, hk, len) : -1;
+    const T* kp = (const T*)p.kpool; const T* vp = (const T*)p.vpool;
+    const int shift = p.map.shift, mask = (1 << shift) - 1;
+    const int* table = p.map.table + (long)b * p.map.ld;
+
+    // page numbers of a step's slots: k the K rows of this lane (slot tile * 16 + li), v its four S / V slots (tile * 16 + 4 g)
+    struct Pages { int k[NT], v[NT]; };
+    auto fetch = [&](int s0, Pages& e) {
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            e.k[t] = table[min((s0 + t * 16 + li) >> shift, p.map.width - 1)];
+            e.v[t] = table[min((s0 + t * 16 + g * 4) >> shift, p.map.width - 1)];
+        }
+    };
+    auto row_of = [&](int e, int slot) -> long {                                        // slots that do not exist read row 0 of the pool and weigh nothing
+        const bool ok = slot < hi && (unsigned)e < (unsigned)p.map.n_pages;
+        return ok ? (((long)e * p.Hkv + hk) << shift) + (slot & mask) : 0;
+    };
+    S_t st;
+    auto load_k = [&](int s0, const Pages& e) {
+        long r[NT];
+#pragma unroll
+        for (int t = 0; t < NT; t++) r[t] = row_of(e.k[t], s0 + t * 16 + li);
+        st.load_k(kp, r, d, g);
+    };
+    unsigned ok = 0;                                                                    // bit t * 4 + i: slot exists
+    long vrow[NT];
+    auto load_v = [&](int s0, const Pages& e) {
+        ok = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            vrow[t] = row_of(e.v[t], s0 + t * 16 + g * 4);
+            const int left = hi - (s0 + t * 16 + g * 4);
+            if ((unsigned)e.v[t] < (unsigned)p.map.n_pages && left > 0) ok |= (left >= 4 ? 15u : (1u << left) - 1u) << (t * 4);
+        }
+        st.load_v(vp, vrow, d, li);
+    };
+    Pages e0, e1;
+    int s0 = lo + wave * ST;
+    const bool any = s0 < hi;                                                           // wave-uniform
+    if (any) {
+        fetch(s0, e0);
+        load_k(s0, e0);
+        load_v(s0, e0);
+        fetch(s0 + RD, e1);
+    }
+    // ---- q (and the new key), rotated, while the first rows are under way
+    const long trow = (long)paged_pos(p.positions, p.lengths, p.kn != nullptr, p.n_pos, b) * (p.rot >> 1);
+    const float* cs = p.cos_t + trow; const float* sn = p.sin_t + trow;
+    if (nh < 16 || d < DP)
+        for (int i = tid; i < QB / 16; i += 256) *reinterpret_cast<u4_t*>(lds + i * 16) = u4_t{0u, 0u, 0u, 0u};
+    if (mine && d < DP) for (int c = d + tid; c < DP; c += 256) own_k[c] = own_v[c] = from_f<T>(0.f);
+    if (nh < 16 || d < DP) lds_barrier();
+    for (int i = tid; i < nh * d; i += 256) {
+        const int h = i / d, c = i - h * d;
+        S_t::put_q(lds, h, c, rotated((const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d, c, p.rot, cs, sn));
+    }
+    if (mine)
+        for (int c = tid; c < d; c += 256) {
+            const T kv = from_f<T>(rotated((const T*)p.kn + (long)b * p.ld_k + (long)hk * d, c, p.rot, cs, sn));
+            const T vv = ((const T*)p.vn)[(long)b * p.ld_v + (long)hk * d + c];
+            own_k[c] = kv; own_v[c] = vv;
+            if (own_row >= 0 && ct == 0) { ((T*)p.kpool)[own_row * d + c] = kv; ((T*)p.vpool)[own_row * d + c] = vv; }
+        }
+    lds_barrier();
+    st.get_q(lds, lane);
+
+    f32x4_t acc[NS][VE];
+#pragma unroll
+    for (int s = 0; s < NS; s++)
+#pragma unroll
+        for (int e = 0; e < VE; e++) acc[s][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+    const float sc = p.stable ? p.scale : p.scale * 1.44269504088896340736f;            // softmax in base 2
+    float* srow = p.sc ? p.sc + ((long)b * p.H + h0 + li) * cap : nullptr;
+    // from the scores of a step to its probabilities (relative to the running maximum), which rescale what was gathered before
+    auto weigh = [&](const f32x4_t (&s)[NT], unsigned okb, float (&pr)[J], int slot) {
+        float x[J];
+#pragma unroll
+        for (int j = 0; j < J; j++) x[j] = s[j >> 2][j & 3] * sc;
+        if (srow && li < nh) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+                const unsigned bits = okb >> (t * 4) & 15;
+                if (slot >= 0 && bits == 15) *reinterpret_cast<f32x4_t*>(srow + slot + t * 16 + g * 4) = f32x4_t{x[t * 4], x[t * 4 + 1], x[t * 4 + 2], x[t * 4 + 3]};
+                else if (slot >= 0) {                                                   // the last slots: the new token's score is another wave's
+#pragma unroll
+                    for (int i = 0; i < 4; i++) if (bits >> i & 1) srow[slot + t * 16 + g * 4 + i] = x[t * 4 + i];
+                } else if (bits) srow[len] = x[0];
+            }
+        }
+        if (p.stable) {
+#pragma unroll
+            for (int j = 0; j < J; j++) { pr[j] = okb >> j & 1 ? stable_s(x[j]) : 0.f; l += pr[j]; }
+            return;
+        }
+        float mx = m;
+#pragma unroll
+        for (int j = 0; j < J; j++) { x[j] = okb >> j & 1 ? x[j] : -INFINITY; mx = fmaxf(mx, x[j]); }
+        mx = quad_max(mx);
+        const float base = mx == -INFINITY ? 0.f : mx;
+        const float al = __builtin_amdgcn_exp2f(m - base);
+        if (__ballot(mx != m)) {                                                        // someone's maximum grew
+            l *= al;
+#pragma unroll
+            for (int a = 0; a < NS; a++)
+#pragma unroll
+                for (int e = 0; e < VE; e++) acc[a][e] *= al;
+        }
+        m = mx;
+#pragma unroll
+        for (int j = 0; j < J; j++) { pr[j] = okb >> j & 1 ? __builtin_amdgcn_exp2f(x[j] - base) : 0.f; l += pr[j]; }
+    };
+    f32x4_t s[NT];
+    float pr[J];
+    const bool trim = d < DP;
+    if (any) {
+        for (; s0 + RD < hi; s0 += RD) {
+            if (trim) st.trim_k(d, g);
+            st.scores(lds, lane, p.rot, s);
+            load_k(s0 + RD, e1);
+            weigh(s, ok, pr, s0);
+            st.gather(pr, ok, vp, vrow, d, li, acc);
+            load_v(s0 + RD, e1);
+            fetch(s0 + 2 * RD, e1);
+        }
+        if (trim) st.trim_k(d, g);
+        st.scores(lds, lane, p.rot, s);
+        weigh(s, ok, pr, s0);
+        st.gather(pr, ok, vp, vrow, d, li, acc);
+    }
+    if (mine && own_row >= 0 && wave == (n - lo + ST - 1) / ST % 4) {                   // the new token: the wave whose turn it is
+        st.own_k(own_k, li, g);
+        st.scores(lds, lane, p.rot, s);
+        weigh(s, lane < 16 ? 1u : 0u, pr, -1);
+        st.gather_own(pr, own_v, li, g, acc);
+    }
+    // ---- the four waves' parts; a wave without slots has m = -inf, l = 0 and weighs nothing
+    l = quad_sum(l);
+    if (g == 0) { st_m[wave][li] = m; st_l[wave][li] = l; }
+    lds_barrier();                                                                      // also: the q fragments have been read
+    float M = 0.f, L = 0.f, f = 1.f;
+    if (!p.stable) {
+        M = fmaxf(fmaxf(st_m[0][li], st_m[1][li]), fmaxf(st_m[2][li], st_m[3][li]));
+        const float base = M == -INFINITY ? 0.f : M;
+#pragma unroll
+        for (int w = 0; w < 4; w++) L += st_l[w][li] * __builtin_amdgcn_exp2f(st_m[w][li] - base);
+        f = __builtin_amdgcn_exp2f(m - base);
+    } else {
+#pragma unroll
+        for (int w = 0; w < 4; w++) L += st_l[w][li];
+    }
+    const bool single = p.nsplit == 1;
+    if (p.stat && wave == 0 && g == 0 && li < nh) p.stat[((long)b * p.H + h0 + li) * p.nsplit + split] = make_float2(M, L);
+    if (single) f *= p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
+    float* out = (float*)lds;
+#pragma unroll
+    for (int a = 0; a < NS; a++) {
+        if (a) lds_barrier();
+        if (li < nh)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < VE; e += 4)
+                    *reinterpret_cast<f32x4_t*>(out + (wave * 16 + li) * SW + (g * 4 + r) * VE + e) =
+                        f32x4_t{acc[a][e][r] * f, acc[a][e + 1][r] * f, acc[a][e + 2][r] * f, acc[a][e + 3][r] * f};
+        lds_barrier();
+        for (int i = tid; i < nh * (SW / 4); i += 256) {
+            const int h = i / (SW / 4), c = (i % (SW / 4)) * 4;
+            if (a * SW + c >= d) continue;
+            f32x4_t v = *reinterpret_cast<f32x4_t*>(out + h * SW + c);
+#pragma unroll
+            for (int w = 1; w < 4; w++) v += *reinterpret_cast<f32x4_t*>(out + (w * 16 + h) * SW + c);
+            const float r[4] = {v[0], v[1], v[2], v[3]};
+            const long bh = (long)b * p.H + h0 + h;
+            if (single) VecIO<T, 4>::store((T*)p.o + bh * d + a * SW + c, r);
+            else VecIO<float, 4>::store(p.part + (bh * p.nsplit + split) * d + a * SW + c, r);
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ joining the splits, adding the weights up
+__device__ __forceinline__ int paged_cover(const PagedP& p, int b) {
+    const int len = p.lengths[b], cap = p.map.capacity();
+    return len < 0 ? 0 : min(min(len, cap) + (p.kn ? 1 : 0), cap);
+}
+// Workgroups below `joins`: one (row, head): the splits' outputs, 256 / (d / 4) of them at a time, d / 4 lanes of 16 bytes each.
+// The others: 1024 slots of one (row, KV head): p = exp2(x - max) / sum (| s(x) / sum) of the group's heads, added to the slots' weights.
+template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const PagedP p, int joins, int wchunks) {
+    __shared__ __attribute__((aligned(16))) float red[256 * 4];
+    __shared__ float red_l[256];
+    const int tid = threadIdx.x;
+    if ((int)blockIdx.x < joins) {
+        const int bh = blockIdx.x, b = bh / p.H, cols = p.d >> 2, per = 256 / cols;
+        const int c = tid % cols, gr = tid / cols;
+        const int ns = (paged_cover(p, b) + p.chunk - 1) / p.chunk;
+        const float2* st = p.stat + (long)bh * p.nsplit;
+        float M = -INFINITY;
+        if (!p.stable) for (int s = 0; s < ns; s++) M = fmaxf(M, st[s].x);
+        const float base = p.stable || M == -INFINITY ? 0.f : M;
+        f32x4_t a = {0.f, 0.f, 0.f, 0.f};
+        float L = 0.f;
+        if (gr < per)
+            for (int s = gr; s < ns; s += per) {
+                const float f = p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base);
+                L = fmaf(st[s].y, f, L);
+                a += *reinterpret_cast<const f32x4_t*>(p.part + ((long)bh * p.nsplit + s) * p.d + c * 4) * f;
+            }
+        *reinterpret_cast<f32x4_t*>(red + tid * 4) = a;
+        red_l[tid] = L;
+        __syncthreads();
+        if (gr == 0) {
+            for (int k = 1; k < per; k++) { a += *reinterpret_cast<f32x4_t*>(red + (k * cols + c) * 4); L += red_l[k * cols + c]; }
+            const float inv = p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
+            const float r[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
+            VecIO<T, 4>::store((T*)p.o + (long)bh * p.d + c * 4, r);
+        }
+        return;
+    }
+    const int id = blockIdx.x - joins, ch = id % wchunks, bk = id / wchunks, b = bk / p.Hkv, hk = bk % p.Hkv;
+    const int n = paged_cover(p, b), s0 = ch * 1024;
+    if (s0 >= n) return;
+    const int ns = (n + p.chunk - 1) / p.chunk, cap = p.map.capacity();
+    const int slot = s0 + tid * 4;
+    f32x4_t add = {0.f, 0.f, 0.f, 0.f};
+    for (int h = 0; h < p.G; h++) {
+        const long bh = (long)b * p.H + hk * p.G + h;
+        const float2* st = p.stat + bh * p.nsplit;
+        float M = -INFINITY, L = 0.f;
+        if (!p.stable) for (int s = 0; s < ns; s++) M = fmaxf(M, st[s].x);
+        const float base = p.stable || M == -INFINITY ? 0.f : M;
+        for (int s = 0; s < ns; s++) L = fmaf(st[s].y, p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base), L);
+        const float inv = p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
+        if (slot < n) {
+            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.sc + bh * cap + slot);
+#pragma unroll
+            for (int i = 0; i < 4; i++) add[i] += (p.stable ? stable_s(x[i]) : __builtin_amdgcn_exp2f(x[i] - base)) * inv;
+        }
+    }
+    if (slot >= n) return;
+    const long row = p.map.row(b, hk, slot);                                            // four slots of one page (page >= 4)
     if (row < 0) return;
-    const long t = (long)paged_pos(p, b) * (p.rot >> 1);
-    const T* k = (const T*)p.kn + (long)b * p.ld_k + (long)h * p.d;
-    const T* v = (const T*)p.vn + (long)b * p.ld_v + (long)h * p.d;
-    for (int c = threadIdx.x; c < p.d; c += 64) {
-        ((T*)p.kpool)[row * p.d + c] = from_f<T>(rotated(k, c, p.rot, p.cos_t + t, p.sin_t + t));
-        ((T*)p.vpool)[row * p.d + c] = v[c];
-    }
-    if (p.w && threadIdx.x == 0) p.w[row] = 0.f;
+    const int len = p.lengths[b];
+#pragma unroll
+    for (int i = 0; i < 4; i++)
+        if (slot + i < n) p.w[row + i] = p.kn && slot + i == len ? add[i] : p.w[row + i] + add[i];
 }
 
-__device__ __forceinline__ float block_max(float v, float* red) {
-    for (int i = 1; i < 64; i <<= 1) v = fmaxf(v, __shfl_xor(v, i));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+// How a cache of `cap` slots is split.  A workgroup takes whole rounds of 128 slots.
+static int paged_chunk(int64_t tiles, int64_t cap) {
+    const int64_t want = 1024;
+    int64_t chunk = cdiv(cdiv(cap * tiles, want), 128) * 128;
+    if (chunk > 1024) chunk = 1024;
+    if (cap <= 512) chunk = cap;
+    return (int)(cdiv(chunk, 128) * 128);
 }
-
-template <typename T> __global__ __launch_bounds__(256) void paged_attn_k(const PagedP p, int stable) {
-    __shared__ float qs[512], red[4];
-    const int b = blockIdx.x, h = blockIdx.y, hk = h / p.G;
-    const int n = min(p.lengths[b] < 0 ? 0 : p.lengths[b] + (p.kn ? 1 : 0), p.map.capacity());
-    const long t = (long)paged_pos(p, b) * (p.rot >> 1);
-    float* sc = p.sc + ((long)b * p.H + h) * p.map.capacity();
-    for (int c = threadIdx.x; c < p.d; c += 256)
-        qs[c] = rotated((const T*)p.q + (long)b * p.ld_q + (long)h * p.d, c, p.rot, p.cos_t + t, p.sin_t + t);
-    __syncthreads();
-    float m = -INFINITY;
-    for (int s = threadIdx.x; s < n; s += 256) {
-        const long row = p.map.row(b, hk, s);
-        float x = 0.f;
-        if (row >= 0) {
-            for (int c = 0; c < p.d; c++) x = fmaf(qs[c], to_f(((const T*)p.kpool)[row * p.d + c]), x);
-            x *= p.scale;
-            m = fmaxf(m, x);
-        }
-        sc[s] = x;
-    }
-    m = block_max(m, red);
-    if (m == -INFINITY) m = 0.f;
-    float l = 0.f;
-    for (int s = threadIdx.x; s < n; s += 256) {
-        const bool there = p.map.row(b, hk, s) >= 0;
-        const float x = sc[s];
-        const float e = !there ? 0.f : stable ? (x < 0.f ? 1.f / (1.f - x + 1e-9f) : x + 1.f) : expf(x - m);
-        sc[s] = e;
-        l += e;
-    }
-    __syncthreads();
-    l = block_sum<4>(l, red);
-    const float inv = stable ? 1.f / fmaxf(l, 1e-9f) : l == 0.f ? 0.f : 1.f / l;
-    __threadfence_block();
-    __syncthreads();
-    for (int c = threadIdx.x; c < p.d; c += 256) {
-        float a = 0.f;
-        for (int s = 0; s < n; s++) {
-            const long row = p.map.row(b, hk, s);
-            if (row >= 0) a = fmaf(sc[s], to_f(((const T*)p.vpool)[row * p.d + c]), a);
-        }
-        ((T*)p.o)[((long)b * p.H + h) * p.d + c] = from_f<T>(a * inv);
-    }
-    __syncthreads();
-    for (int s = threadIdx.x; s < n; s += 256) sc[s] *= inv;
-}
-__global__ __launch_bounds__(256) void paged_weights_k(const PagedP p) {
-    const int b = blockIdx.x, hk = blockIdx.y;
-    const int n = min(p.lengths[b] < 0 ? 0 : p.lengths[b] + (p.kn ? 1 : 0), p.map.capacity());
-    for (int s = threadIdx.x; s < n; s += 256) {
-        const long row = p.map.row(b, hk, s);
-        if (row < 0) continue;
-        float a = 0.f;
-        for (int g = 0; g < p.G; g++) a += p.sc[((long)b * p.H + hk * p.G + g) * p.map.capacity() + s];
-        p.w[row] += a;
-    }
+struct PagedPlan { int chunk, nsplit; size_t part, stat, sc; };
+static PagedPlan paged_plan(const mm_paged_attn_args* a) {
+    const int64_t cap = a->width * a->page, tiles = a->B * a->Hkv * cdiv(a->H / a->Hkv, 16);
+    PagedPlan r;
+    r.chunk = paged_chunk(tiles, cap);
+    r.nsplit = (int)cdiv(cap, r.chunk);
+    r.part = r.nsplit > 1 ? (size_t)(a->B * a->H) * r.nsplit * a->d * sizeof(float) : 0;
+    r.stat = r.nsplit > 1 || a->weights ? (size_t)(a->B * a->H) * r.nsplit * sizeof(float2) : 0;
+    r.stat = (r.stat + 15) / 16 * 16;
+    r.sc = a->weights ? (size_t)(a->B * a->H) * cap * sizeof(float) : 0;
+    return r;
 }
 
 extern "C" size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* a) {
-    if (!a || a->B <= 0 || a->H <= 0 || a->width <= 0 || a->page <= 0) return 0;
-    return (size_t)a->B * a->H * a->width * a->page * sizeof(float);
+    if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->H < a->Hkv || a->d <= 0 || a->width <= 0 || a->page <= 0) return 0;
+    const PagedPlan r = paged_plan(a);
+    return r.part + r.stat + r.sc;
+}
+
+template <typename T, int VE, int NS, int NT, bool AL8> static void paged_launch(const PagedP& p, unsigned blocks, hipStream_t st) {
+    hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL8>), dim3(blocks), dim3(256), 0, st, p);
 }
 
 extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
@@ -115,51 +542,99 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     if (a->B == 0) return MM_OK;
     MM_CHECK(a->q && a->o && a->lengths && (!a->k_new == !a->v_new), "paged_decode_attn: null pointer");
     MM_CHECK(a->H > 0 && a->H <= 65535 && a->H % a->Hkv == 0, "paged_decode_attn: %lld query heads over %lld KV heads", (long long)a->H, (long long)a->Hkv);
-    MM_CHECK(a->rot >= 0 && a->rot <= a->d && a->rot % 2 == 0 && (a->rot == 0 || (a->cos_t && a->sin_t && a->n_pos > 0)), "paged_decode_attn: bad rot/tables");
+    MM_CHECK(a->rot >= 0 && a->rot <= a->d && a->rot % 2 == 0 && (a->rot == 0 || (a->cos_t && a->sin_t && a->n_pos > 0 && a->n_pos < (1LL << 31))),
+             "paged_decode_attn: bad rot/tables");
     MM_CHECK(a->ld_q >= 0 && a->ld_k >= 0 && a->ld_v >= 0, "paged_decode_attn: negative row stride");
     MM_CHECK(a->mode == MM_ATTN_SOFTMAX || a->mode == MM_ATTN_STABLEMAX, "paged_decode_attn: bad mode %d", a->mode);
-    MM_CHECK(a->workspace && a->workspace_bytes >= mm_paged_decode_attn_workspace(a), "paged_decode_attn: workspace too small");
+    MM_CHECK(((uintptr_t)a->o % 16) == 0, "paged_decode_attn: o must be 16-byte aligned");
+    const PagedPlan r = paged_plan(a);
+    const size_t need = r.part + r.stat + r.sc;
+    MM_CHECK(need == 0 || (a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0), "paged_decode_attn: workspace too small or not 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     PagedP p{};
     p.q = a->q; p.kn = a->k_new; p.vn = a->v_new; p.kpool = a->kpool; p.vpool = a->vpool; p.o = a->o; p.w = a->weights;
-    p.lengths = a->lengths; p.positions = a->positions; p.cos_t = a->cos_t; p.sin_t = a->sin_t; p.sc = (float*)a->workspace;
+    p.lengths = a->lengths; p.positions = a->positions; p.cos_t = a->cos_t; p.sin_t = a->sin_t;
     p.map = {a->page_table, (long)a->ld_table, (int)a->width, paged_shift(a->page), (int)a->n_pages, (int)a->Hkv};
+    char* ws = (char*)a->workspace;
+    p.part = r.part ? (float*)ws : nullptr; p.stat = r.stat ? (float2*)(ws + r.part) : nullptr; p.sc = r.sc ? (float*)(ws + r.part + r.stat) : nullptr;
     p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.G = (int)(a->H / a->Hkv); p.d = (int)a->d; p.rot = (int)a->rot;
     p.n_pos = a->rot ? (int)a->n_pos : 1; p.ld_q = a->ld_q; p.ld_k = a->ld_k; p.ld_v = a->ld_v; p.scale = (float)(1.0 / sqrt((double)a->d));
-    const dim3 gk((unsigned)a->B, (unsigned)a->Hkv), gh((unsigned)a->B, (unsigned)a->H);
-    const bool bf = a->dtype == MM_BF16;
-    if (a->k_new) {
-        if (bf) hipLaunchKernelGGL(paged_append_k<bf16>, gk, dim3(64), 0, st, p);
-        else hipLaunchKernelGGL(paged_append_k<float>, gk, dim3(64), 0, st, p);
-        MM_LAUNCH_CHECK();
+    p.chunk = r.chunk; p.nsplit = r.nsplit; p.ctiles = (int)cdiv(p.G, 16); p.stable = a->mode == MM_ATTN_STABLEMAX;
+    const int64_t blocks = a->B * a->Hkv * p.ctiles * p.nsplit;
+    const int wchunks = a->weights ? (int)cdiv(a->width * a->page, 1024) : 0, joins = p.nsplit > 1 ? (int)(a->B * a->H) : 0;
+    const int64_t blocks2 = joins + a->B * a->Hkv * wchunks;
+    MM_CHECK(a->B * a->H < (1LL << 31) && blocks < (1LL << 31) && blocks2 < (1LL << 31), "paged_decode_attn: too many rows and heads for one call");
+    const unsigned nb = (unsigned)blocks;
+    const int64_t d = a->d;
+    if (a->dtype == MM_F32) {
+        if (d <= 64) paged_launch<float, 4, 1, 2, true>(p, nb, st);
+        else if (d <= 128) paged_launch<float, 4, 2, 2, true>(p, nb, st);
+        else if (d <= 192) paged_launch<float, 4, 3, 2, true>(p, nb, st);
+        else if (d <= 256) paged_launch<float, 4, 4, 2, true>(p, nb, st);
+        else paged_launch<float, 4, 8, 1, true>(p, nb, st);
+    } else if (d % 8 == 0) {
+        if (d <= 64) paged_launch<bf16, 4, 1, 2, true>(p, nb, st);
+        else if (d <= 128) paged_launch<bf16, 8, 1, 2, true>(p, nb, st);
+        else if (d <= 192) paged_launch<bf16, 4, 3, 2, true>(p, nb, st);
+        else if (d <= 256) paged_launch<bf16, 8, 2, 2, true>(p, nb, st);
+        else paged_launch<bf16, 8, 4, 2, true>(p, nb, st);
+    } else {                                                                            // rows of whole 8-byte pieces only
+        if (d <= 64) paged_launch<bf16, 4, 1, 2, false>(p, nb, st);
+        else if (d <= 128) paged_launch<bf16, 4, 2, 2, false>(p, nb, st);
+        else if (d <= 192) paged_launch<bf16, 4, 3, 2, false>(p, nb, st);
+        else if (d <= 256) paged_launch<bf16, 4, 4, 2, false>(p, nb, st);
+        else paged_launch<bf16, 4, 8, 2, false>(p, nb, st);
     }
-    if (bf) hipLaunchKernelGGL(paged_attn_k<bf16>, gh, dim3(256), 0, st, p, a->mode);
-    else hipLaunchKernelGGL(paged_attn_k<float>, gh, dim3(256), 0, st, p, a->mode);
     MM_LAUNCH_CHECK();
-    if (a->weights) {
-        hipLaunchKernelGGL(paged_weights_k, gk, dim3(256), 0, st, p);
+    if (blocks2) {
+        if (a->dtype == MM_F32) hipLaunchKernelGGL(paged_join_k<float>, dim3((unsigned)blocks2), dim3(256), 0, st, p, joins, wchunks);
+        else hipLaunchKernelGGL(paged_join_k<bf16>, dim3((unsigned)blocks2), dim3(256), 0, st, p, joins, wchunks);
         MM_LAUNCH_CHECK();
     }
     return MM_OK;
 }
 
 // ------------------------------------------------------------------------------------------------ runs of keys and values
+// A copy: keys and values are read once and written once (4 bytes moved per bf16 value and tensor), which HBM bounds.  A lane moves VE
+// consecutive values of one head of one token; for a rotated key it also reads the partner values (the other half: in the same
+// row, so from the cache that has just fetched it), which spares an exchange between lanes.  VE = 8 (bf16) or 4 (f32) where head_dim,
+// rot / 2 and the strides are multiples of it and the rows are aligned, else 1.
 struct FillP {
     const void* k; const void* v; void* kpool; void* vpool; float* w; const int* start; const int* counts; const int* positions;
     const float* cos_t; const float* sin_t; PagedMap map; int S, Hkv, d, rot, n_pos; long ld_k, bs_k, ld_v, bs_v;
 };
-template <typename T> __global__ __launch_bounds__(256) void paged_fill_k(const FillP p) {
+template <typename T, int VE> __global__ __launch_bounds__(256) void paged_fill_k(const FillP p) {
     const int b = blockIdx.y;
-    const long idx = (long)blockIdx.x * 256 + threadIdx.x;              // over [S][Hkv][d]
-    const int c = (int)(idx % p.d), h = (int)(idx / p.d % p.Hkv), s = (int)(idx / ((long)p.d * p.Hkv));
+    const unsigned pieces = (unsigned)p.d / VE, per = pieces * (unsigned)p.Hkv;
+    const unsigned idx = blockIdx.x * 256u + threadIdx.x;                // over [S][Hkv][d / VE]; fits (checked by the launch)
+    const int s = (int)(idx / per);
+    const unsigned rem = idx - (unsigned)s * per;
+    const int h = (int)(rem / pieces), c = (int)(rem - (unsigned)h * pieces) * VE;
     const int st = p.start ? p.start[b] : 0, n = p.counts ? min(p.counts[b], p.S) : p.S;
-    if (st < 0 || s >= n) return;
+    if (st < 0 || s >= n || s > 0x7fffffff - st) return;
+    const T* k = (const T*)p.k + (long)b * p.bs_k + (long)s * p.ld_k + (long)h * p.d;
+    const T* v = (const T*)p.v + (long)b * p.bs_v + (long)s * p.ld_v + (long)h * p.d;
+    float x[VE], y[VE];
+    VecIO<T, VE>::load(k + c, x);
+    VecIO<T, VE>::load(v + c, y);
+    const int half = p.rot >> 1;
+    if (c < p.rot) {
+        const bool low = c < half;
+        const int i = low ? c : c - half;
+        const long pos = p.positions ? (long)p.positions[b] + s : (long)st + s;
+        const long t = min(max(pos, 0L), (long)p.n_pos - 1) * half + i;
+        float o[VE];
+        VecIO<T, VE>::load(k + (low ? c + half : i), o);
+#pragma unroll
+        for (int e = 0; e < VE; e++) {
+            const float cs = p.cos_t[t + e], sn = p.sin_t[t + e];
+            x[e] = low ? fmaf(x[e], cs, -(o[e] * sn)) : fmaf(x[e], cs, o[e] * sn);
+        }
+    }
     const long row = p.map.row(b, h, st + s);
     if (row < 0) return;
-    const long t = (long)min(max((p.positions ? p.positions[b] : st) + s, 0), p.n_pos - 1) * (p.rot >> 1);
-    const T* k = (const T*)p.k + (long)b * p.bs_k + (long)s * p.ld_k + (long)h * p.d;
-    ((T*)p.kpool)[row * p.d + c] = from_f<T>(rotated(k, c, p.rot, p.cos_t + t, p.sin_t + t));
-    ((T*)p.vpool)[row * p.d + c] = ((const T*)p.v)[(long)b * p.bs_v + (long)s * p.ld_v + (long)h * p.d + c];
+    VecIO<T, VE>::store((T*)p.kpool + row * p.d + c, x);
+    VecIO<T, VE>::store((T*)p.vpool + row * p.d + c, y);
     if (p.w && c == 0) p.w[row] = 0.f;
 }
 
@@ -170,18 +645,28 @@ extern "C" int mm_paged_cache_fill(const mm_paged_fill_args* a, void* stream) {
     MM_CHECK(a->S >= 0 && a->S < (1LL << 30), "paged_cache_fill: S=%lld", (long long)a->S);
     if (a->B == 0 || a->S == 0) return MM_OK;
     MM_CHECK(a->k && a->v, "paged_cache_fill: null pointer");
-    MM_CHECK(a->rot >= 0 && a->rot <= a->d && a->rot % 2 == 0 && (a->rot == 0 || (a->cos_t && a->sin_t && a->n_pos > 0)), "paged_cache_fill: bad rot/tables");
+    MM_CHECK(a->rot >= 0 && a->rot <= a->d && a->rot % 2 == 0 && (a->rot == 0 || (a->cos_t && a->sin_t && a->n_pos > 0 && a->n_pos < (1LL << 31))),
+             "paged_cache_fill: bad rot/tables");
     MM_CHECK(a->ld_k >= 0 && a->ld_v >= 0 && a->bs_k >= 0 && a->bs_v >= 0, "paged_cache_fill: negative stride");
     FillP p{};
     p.k = a->k; p.v = a->v; p.kpool = a->kpool; p.vpool = a->vpool; p.w = a->weights; p.start = a->start; p.counts = a->counts; p.positions = a->positions;
     p.cos_t = a->cos_t; p.sin_t = a->sin_t; p.map = {a->page_table, (long)a->ld_table, (int)a->width, paged_shift(a->page), (int)a->n_pages, (int)a->Hkv};
     p.S = (int)a->S; p.Hkv = (int)a->Hkv; p.d = (int)a->d; p.rot = (int)a->rot; p.n_pos = a->rot ? (int)a->n_pos : 1;
     p.ld_k = a->ld_k; p.bs_k = a->bs_k; p.ld_v = a->ld_v; p.bs_v = a->bs_v;
-    const int64_t per = a->S * a->Hkv * a->d;
-    MM_CHECK(cdiv(per, 256) < (1LL << 31), "paged_cache_fill: too many tokens");
-    const dim3 grid((unsigned)cdiv(per, 256), (unsigned)a->B);
-    if (a->dtype == MM_BF16) hipLaunchKernelGGL(paged_fill_k<bf16>, grid, dim3(256), 0, (hipStream_t)stream, p);
-    else hipLaunchKernelGGL(paged_fill_k<float>, grid, dim3(256), 0, (hipStream_t)stream, p);
+    const int VE = a->dtype == MM_BF16 ? 8 : 4;
+    const int64_t all = a->d | a->rot / 2 | a->ld_k | a->bs_k | a->ld_v | a->bs_v;
+    const bool wide = all % VE == 0 && (((uintptr_t)a->k | (uintptr_t)a->v) % 16) == 0;
+    const int64_t items = a->S * a->Hkv * (a->d / (wide ? VE : 1));
+    MM_CHECK(items < (1LL << 31), "paged_cache_fill: too many tokens for one call");
+    const dim3 grid((unsigned)cdiv(items, 256), (unsigned)a->B);
+    hipStream_t st = (hipStream_t)stream;
+    if (a->dtype == MM_BF16) {
+        if (wide) hipLaunchKernelGGL((paged_fill_k<bf16, 8>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_fill_k<bf16, 1>), grid, dim3(256), 0, st, p);
+    } else {
+        if (wide) hipLaunchKernelGGL((paged_fill_k<float, 4>), grid, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((paged_fill_k<float, 1>), grid, dim3(256), 0, st, p);
+    }
     MM_LAUNCH_CHECK();
     return MM_OK;
 }

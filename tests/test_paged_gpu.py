@@ -5,7 +5,8 @@ Tolerances, fixed before any run, for one output element of attention over n slo
   + E * sum_s p_s |v_s|, where E bounds the relative error of a probability and of the weighted sum:
       the score: d products and d sums in f32, (d + 8) 2^-24 of sum |q k| / sqrt(d) =: (d + 8) 2^-24 M; it enters p once directly and once
       through the normaliser;   exp / reciprocal and their arguments, 16 2^-24;   n + 8 roundings of each of the two sums;
-      bf16: p is used as two bf16 terms (2^-16) and the rotated q as three (2^-24).
+      bf16: p is used as two bf16 terms, the first truncated (it leaves less than 2^-7 p, of which rounding the second loses 2^-8: 2^-15),
+      and the rotated q as three truncated ones (8 bits each: 24, exact).
 Stored keys: half a step of the type times the value + 4 2^-24 (|a| + |b|) of the pair that is rotated.  The attention reference
 reads the keys as stored, which is what the operator is defined on.  Everything that is only moved is compared bit by bit."""
 import math
@@ -88,7 +89,7 @@ def _attend(q, K, V, there, stable, dtype):
         p = torch.softmax(x.masked_fill(~there, -math.inf), -1)
     o = (p[..., None] * V).sum(1)
     E = 2 * (d + 8) * U * M + 16 * U + 2 * (n + 8) * U
-    tol = HALF[dtype] * o.abs() + (E + (2.0 ** -16 if dtype == torch.bfloat16 else 0.0)) * (1 + 2.0 ** -7) * (p[..., None] * V.abs()).sum(1)
+    tol = HALF[dtype] * o.abs() + (E + (2.0 ** -15 if dtype == torch.bfloat16 else 0.0)) * (1 + 2.0 ** -7) * (p[..., None] * V.abs()).sum(1)
     return o, tol, p, E + U
 
 
@@ -261,6 +262,26 @@ def test_non_finite_slots_that_count_and_that_do_not():
         assert torch.isfinite(o[0]).all() and torch.isnan(o[1]).all()
         o2 = o[2].view(2, 64)
         assert torch.isinf(o2[:, 9]).all() and torch.isfinite(torch.cat((o2[:, :9], o2[:, 10:]), 1)).all()
+
+
+def test_an_infinite_key_weighs_nothing_or_everything():
+    """A key with -inf where q is positive scores -inf: weight 0, the row as without it (rotated q: three terms, none of them 0)."""
+    from multimodal_amd import ops
+    for dtype in (torch.bfloat16, torch.float32):
+        c, q, k, v = _filled(18, dtype, 1, 1, 1, 64, 16, [50])
+        n = torch.tensor([50], dtype=torch.int32, device=DEV)
+        q = q.abs().clone()
+        q[0, 40] = 1.5                                                                    # exact in one term
+        tabs = _tables(64, 51)
+        tabs = (tabs[0].clone().fill_(1.0), tabs[1].clone().fill_(0.0))                   # a rotation by nothing
+        for col in (40, 7):
+            c.k[int(c.table[0, 1]), 0, 5] = 0
+            c.k[int(c.table[0, 1]), 0, 5, col] = -math.inf
+            o = ops.paged_decode_attn(q, k, v, c.k, c.v, c.table, n, 1, 64, *tabs, False)
+            K, V = c.rows(c.k, 0, 51), c.rows(c.v, 0, 51)
+            keep = torch.arange(51) != 21
+            want, tol, _, _ = _attend(q[0].double().cpu().view(1, 64), K[:, keep], V[:, keep], torch.ones(50, dtype=torch.bool), False, dtype)
+            assert ((o.double().cpu().view(1, 64) - want).abs() <= tol).all()
 
 
 def test_large_scores_do_not_overflow():
