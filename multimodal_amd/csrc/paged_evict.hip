@@ -1,90 +1,283 @@
 // Eviction from a paged key-value cache by accumulated attention weight (include/mmhip.h).
+//
+// Per (row, KV head): the A = budget - recent greatest of `old` weights, then as few moves as possible.  Attention does not ask for an
+// order of the slots, so survivors among the first A slots stay; the i-th hole there takes the i-th survivor from behind.  Sources (>= A)
+// and targets (< A) are disjoint: all moves are independent.  The newest slots then shift down by n - budget; a slot's target is the
+// source of the slot n - budget before it, so the slots of one residue class mod n - budget form a chain, and a thread that walks its
+// chain in order needs no one else.  HBM bounds the moves: 4 d values per slot moved (K and V, read and written).
+//
+// Selection: weights as ordered 32-bit keys, the A-th greatest found bit by bit from the top: count the keys >= candidate by ballots
+// (no atomics: a histogram's bins collide where weights are alike, and equal weights are the rule at the start).  Up to 65536 slots stay
+// in registers, longer rows are read again in every pass.
 #include "paged.h"
 
-// Order of weights as unsigned integers: greater weight, greater key; NaN above everything, -0 = 0, a slot that does not exist lowest.
+// Order of weights as unsigned integers: greater weight, greater key; NaN above everything, -0 = 0, a slot that does not exist lowest (0).
 __device__ __forceinline__ unsigned weight_key(float x) {
     if (x != x) return 0xffffffffu;
     const unsigned u = __float_as_uint(x == 0.f ? 0.f : x);
     return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 struct EvictP {
-    void* kpool; void* vpool; float* w; int* lengths; int* kept; PagedMap map; unsigned* keys; int d, es, budget, recent;
+    char* kpool; char* vpool; float* w; int* lengths; int* kept; PagedMap map;
+    int* ws;                       // per (row, KV head): {slots, moves}, then targets [room] and sources [room] of the moves
+    int room, units, budget, recent, B;                                        // units: 16- or 8-byte pieces of a slot's K
+    __device__ __forceinline__ int* head(long bh) const { return ws + bh * (2L * room + 4); }
 };
-__device__ __forceinline__ void move_slot(const EvictP& p, long to, long from, int lane, int lanes) {
-    if (to < 0 || from < 0) return;
-    const int n4 = p.d * p.es / 4;                                     // d % 4 == 0: whole 4-byte words (8 in bf16)
-    const unsigned* ks = (const unsigned*)p.kpool + from * n4; unsigned* kd = (unsigned*)p.kpool + to * n4;
-    const unsigned* vs = (const unsigned*)p.vpool + from * n4; unsigned* vd = (unsigned*)p.vpool + to * n4;
-    for (int i = lane; i < n4; i += lanes) { kd[i] = ks[i]; vd[i] = vs[i]; }
-    if (lane == 0) p.w[to] = p.w[from];
+
+// ------------------------------------------------------------------------------------------------ selection (NW waves)
+template <int NW> __device__ __forceinline__ int block_count(int c, int* red, int& buf) {       // c: wave-uniform
+    int* r = red + (buf ^= NW);
+    if ((threadIdx.x & 63) == 0) r[threadIdx.x >> 6] = c;
+    __syncthreads();
+    int t = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) t += r[i];
+    return t;
 }
-// One workgroup per (row, KV head): rank every old slot by counting, list the moves, make them.
-__global__ __launch_bounds__(256) void paged_evict_k(const EvictP p) {
-    const int b = blockIdx.x, h = blockIdx.y, cap = p.map.capacity(), tid = threadIdx.x;
-    const int n = min(p.lengths[b], cap);
-    int* kept = p.kept + ((long)b * p.map.Hkv + h) * p.budget;
-    if (n <= p.budget) {
-        for (int j = tid; j < p.budget; j += 256) kept[j] = j < n ? j : -1;
-        return;
-    }
-    const int A = p.budget - p.recent, old = n - p.recent;
-    unsigned* key = p.keys + ((long)b * p.map.Hkv + h) * cap;
-    for (int s = tid; s < old; s += 256) { const long r = p.map.row(b, h, s); key[s] = r < 0 ? 0u : weight_key(p.w[r]); }
+// exclusive prefix of v over the workgroup's threads, and the total
+template <int NW> __device__ __forceinline__ int block_scan(int v, int* red, int& buf, int& total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int s = v;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) { const int t = __shfl_up(s, o); if (lane >= o) s += t; }
+    int* r = red + (buf ^= NW);
+    if (lane == 63) r[wave] = s;
     __syncthreads();
-    for (int s = tid; s < A; s += 256) kept[s] = -2;
-    __syncthreads();
-    int* mark = (int*)key;                                             // becomes 1 for survivors behind the kept region (after all ranks)
-    __shared__ int any;
-    // ranks: survivors of the kept region say so in kept[]; those behind it are found again below by the same count
-    for (int s = tid; s < old; s += 256) {
-        int rank = 0;
-        const unsigned mine = key[s];
-        for (int o = 0; o < old; o++) rank += key[o] > mine || (key[o] == mine && o < s);
-        if (s < A && rank < A) kept[s] = s;
-    }
-    __syncthreads();
-    if (tid == 0) any = 0;
-    __syncthreads();
-    for (int s0 = A; s0 < old; s0 += 256) {                            // in order: the i-th survivor takes the i-th hole
-        const int s = s0 + tid;
-        int rank = old;
-        if (s < old) {
-            rank = 0;
-            const unsigned mine = key[s];
-            for (int o = 0; o < old; o++) rank += key[o] > mine || (key[o] == mine && o < s);
-        }
-        __shared__ int late[256];
-        late[tid] = rank < A;
-        __syncthreads();
-        if (tid == 0)
-            for (int i = 0; i < 256; i++)
-                if (late[i]) {
-                    while (kept[any] != -2) any++;
-                    kept[any] = s0 + i;
-                }
-        __syncthreads();
-    }
-    (void)mark;
-    const int wave = tid >> 6, lane = tid & 63;
-    for (int j = wave; j < A; j += 4) if (kept[j] != j) move_slot(p, p.map.row(b, h, j), p.map.row(b, h, kept[j]), lane, 64);
-    __threadfence_block();
-    __syncthreads();
-    for (int j = A; j < p.budget; j++) {                               // the newest slots: down by n - budget, in order
-        move_slot(p, p.map.row(b, h, j), p.map.row(b, h, n - p.budget + j), tid, 256);
-        if (tid == 0) kept[j] = n - p.budget + j;
-        __threadfence_block();
-        __syncthreads();
-    }
-}
-__global__ void paged_lengths_k(int* lengths, int B, int budget, int cap) {
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b < B && min(lengths[b], cap) > budget) lengths[b] = budget;
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int i = 0; i < NW; i++) { before += i < wave ? r[i] : 0; total += r[i]; }
+    return before + s - v;
 }
 
-extern "C" size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page, int64_t width, int64_t budget, int64_t recent) {
-    (void)budget; (void)recent;
-    return (B > 0 && Hkv > 0 && page > 0 && width > 0) ? (size_t)(B * Hkv * page * width) * sizeof(unsigned) : 0;
+// R registers of keys a thread (four consecutive slots a round), R = 0: read again in every pass
+template <int NW, int R> __device__ void evict_select(const EvictP& p, int b, int h, int* red) {
+    constexpr int ROUND = NW * 256;
+    const long bh = (long)b * p.map.Hkv + h;
+    const int tid = threadIdx.x, n = min(p.lengths[b], p.map.capacity());
+    int* kept = p.kept + bh * p.budget;
+    int* hd = p.head(bh);
+    if (tid == 0) { hd[0] = n; hd[1] = 0; }
+    if (n <= p.budget) {
+        for (int j = tid; j < p.budget; j += NW * 64) kept[j] = j < n ? j : -1;
+        return;
+    }
+    const int A = p.budget - p.recent, old = n - p.recent, rounds = (old + ROUND - 1) / ROUND;
+    int* to = hd + 4; int* from = to + p.room;
+    auto load = [&](int r, unsigned (&k)[4]) {
+        const int s = r * ROUND + tid * 4;                                     // four slots of one page
+        const long row = s < old ? p.map.row(b, h, s) : -1;
+        mm_f4_t w = {0.f, 0.f, 0.f, 0.f};
+        if (row >= 0) w = *reinterpret_cast<const mm_f4_t*>(p.w + row);
+#pragma unroll
+        for (int i = 0; i < 4; i++) k[i] = row >= 0 && s + i < old ? weight_key(w[i]) : 0u;
+    };
+    constexpr int RR = R ? R / 4 : 1;
+    unsigned key[RR][4];
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int r = 0; r < RR; r++) load(r, key[r]);
+    }
+    auto count = [&](unsigned t) {                                             // keys >= t (t > 0), over the wave
+        int c = 0;
+        if constexpr (R > 0) {
+#pragma unroll
+            for (int r = 0; r < RR; r++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) c += __popcll(__ballot(key[r][i] >= t));
+        } else {
+            for (int r = 0; r < rounds; r++) {
+                unsigned k[4];
+                load(r, k);
+#pragma unroll
+                for (int i = 0; i < 4; i++) c += __popcll(__ballot(k[i] >= t));
+            }
+        }
+        return c;
+    };
+    int buf = 0, ge = old;                                                     // ge: keys >= T
+    unsigned T = 0;
+    if (A == 0) { T = 0xffffffffu; ge = 0; }                                   // nothing of the old is kept
+    else
+        for (int bit = 31; bit >= 0 && ge != A; bit--) {
+            const unsigned t = T | 1u << bit;
+            const int c = block_count<NW>(count(t), red, buf);
+            if (c >= A) { T = t; ge = c; }
+        }
+    int ties = 0x7fffffff;                                                     // how many keys equal to T are kept, lowest slots first
+    if (A && ge != A) ties = A - (T == 0xffffffffu ? 0 : block_count<NW>(count(T + 1), red, buf));
+    int equal = 0, holes = 0, late = 0;                                        // so far, in slot order
+    auto place = [&](int r, const unsigned (&k)[4]) {
+        const int s = r * ROUND + tid * 4;
+        bool keep[4];
+        int eq = 0, total;
+        if (ties != 0x7fffffff) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) eq += k[i] == T && s + i < old;
+            eq = equal + block_scan<NW>(eq, red, buf, total);
+            equal += total;
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const bool is = k[i] == T && s + i < old;
+            keep[i] = A && s + i < old && (k[i] > T || (is && eq < ties));
+            eq += is;
+        }
+        int c = 0;                                                             // holes | survivors behind A << 16 (a round has at most 4096 slots)
+#pragma unroll
+        for (int i = 0; i < 4; i++) c += s + i < A ? !keep[i] : keep[i] ? 1 << 16 : 0;
+        const int pre = block_scan<NW>(c, red, buf, total);
+        int hole = holes + (pre & 0xffff), sur = late + (int)((unsigned)pre >> 16);
+        holes += total & 0xffff; late += (int)((unsigned)total >> 16);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            if (s + i < A) {
+                if (keep[i]) kept[s + i] = s + i;
+                else { if (hole < p.room) to[hole] = s + i; hole++; }
+            } else if (keep[i]) { if (sur < p.room) from[sur] = s + i; sur++; }
+        }
+    };
+    if constexpr (R > 0) {
+#pragma unroll
+        for (int r = 0; r < RR; r++) if (r < rounds) place(r, key[r]);
+    } else
+        for (int r = 0; r < rounds; r++) { unsigned k[4]; load(r, k); place(r, k); }
+    for (int j = A + tid; j < p.budget; j += NW * 64) kept[j] = n - p.budget + j;
+    __syncthreads();                                                           // the lists are written
+    const int moves = min(holes, late);
+    if (tid == 0) hd[1] = moves;
+    for (int i = tid; i < moves; i += NW * 64) kept[to[i]] = from[i];
 }
+
+// ------------------------------------------------------------------------------------------------ moving
+// independent moves [first, ..) of a (row, KV head), one piece of K and of V a thread; `step` threads share the work
+template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& p, int b, int h, int t, int step) {
+    const int* hd = p.head((long)b * p.map.Hkv + h);
+    const int* to = hd + 4; const int* from = to + p.room;
+    const unsigned total = (unsigned)hd[1] * (unsigned)p.units;
+    U* K = (U*)p.kpool; U* V = (U*)p.vpool;
+    constexpr int N = 4;                                                       // in flight
+    for (unsigned i0 = t; i0 < total; i0 += (unsigned)step * N) {
+        U k[N], v[N];
+        long d[N];
+        int piece[N];
+        float w[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const unsigned i = i0 + (unsigned)(j * step);
+            d[j] = -1;
+            if (i < total) {
+                const unsigned m = i / (unsigned)p.units;
+                piece[j] = (int)(i - m * (unsigned)p.units);
+                const long s = p.map.row(b, h, from[m]);
+                if (s >= 0) {
+                    d[j] = p.map.row(b, h, to[m]);
+                    k[j] = K[s * p.units + piece[j]]; v[j] = V[s * p.units + piece[j]];
+                    if (piece[j] == 0) w[j] = p.w[s];
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (d[j] >= 0) {
+                K[d[j] * p.units + piece[j]] = k[j]; V[d[j] * p.units + piece[j]] = v[j];
+                if (piece[j] == 0) p.w[d[j]] = w[j];
+            }
+    }
+}
+// the newest slots, down by n - budget: one chain (residue class) and piece a thread
+template <typename U> __device__ __forceinline__ void evict_shift(const EvictP& p, int b, int h, int t, int step) {
+    const int n = p.head((long)b * p.map.Hkv + h)[0];
+    if (n <= p.budget) return;
+    const int by = n - p.budget, first = n - p.recent;
+    const unsigned total = (unsigned)min(by, p.recent) * (unsigned)p.units;
+    U* K = (U*)p.kpool; U* V = (U*)p.vpool;
+    constexpr int N = 4;
+    for (unsigned i = t; i < total; i += (unsigned)step) {
+        const unsigned c = i / (unsigned)p.units;
+        const int piece = (int)(i - c * (unsigned)p.units);
+        for (long j0 = c; j0 < p.recent; j0 += (long)N * by) {
+            U k[N], v[N];
+            float w[N];
+            long d[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                const long j = j0 + (long)e * by;
+                d[e] = -1;
+                if (j < p.recent) {
+                    const long s = p.map.row(b, h, first + (int)j);
+                    if (s >= 0) {
+                        d[e] = p.map.row(b, h, first + (int)j - by);
+                        k[e] = K[s * p.units + piece]; v[e] = V[s * p.units + piece];
+                        if (piece == 0) w[e] = p.w[s];
+                    }
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (d[e] >= 0) {
+                    K[d[e] * p.units + piece] = k[e]; V[d[e] * p.units + piece] = v[e];
+                    if (piece == 0) p.w[d[e]] = w[e];
+                }
+        }
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ kernels
+// ALL: select, move and shift in one workgroup per (row, KV head); else the selection alone
+template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW * 64) void evict_select_k(const EvictP p) {
+    __shared__ int red[2 * NW];
+    const int b = blockIdx.x, h = blockIdx.y;
+    evict_select<NW, R>(p, b, h, red);
+    if constexpr (ALL) {
+        __syncthreads();
+        evict_moves<U>(p, b, h, threadIdx.x, NW * 64);
+        __syncthreads();                                                       // targets of the shift were sources of the moves
+        evict_shift<U>(p, b, h, threadIdx.x, NW * 64);
+    }
+}
+template <typename U> __global__ __launch_bounds__(256) void evict_moves_k(const EvictP p) {
+    evict_moves<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
+}
+template <typename U> __global__ __launch_bounds__(256) void evict_shift_k(const EvictP p) {
+    evict_shift<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
+}
+__global__ void evict_lengths_k(const EvictP p) {                              // in a launch of its own: every head's workgroup reads the old ones
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b < p.B && p.lengths[b] > p.budget && p.map.capacity() > p.budget) p.lengths[b] = p.budget;
+}
+
+static int64_t evict_room(int64_t page, int64_t width, int64_t budget, int64_t recent) {
+    const int64_t cap = page * width, A = budget - recent;
+    return cap <= budget ? 0 : A < cap - A ? A : cap - A;                      // moves: at most the holes, at most the survivors behind them
+}
+extern "C" size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page, int64_t width, int64_t budget, int64_t recent) {
+    if (B <= 0 || Hkv <= 0 || page <= 0 || width <= 0 || recent < 0 || budget < recent) return 0;
+    return (size_t)(B * Hkv) * (size_t)(2 * evict_room(page, width, budget, recent) + 4) * sizeof(int);
+}
+
+template <typename U> static void evict_launch(const EvictP& p, int64_t cap, int64_t max_moves, hipStream_t st) {
+    const dim3 grid((unsigned)p.B, (unsigned)p.map.Hkv);
+    const int64_t heads = (int64_t)p.B * p.map.Hkv;
+    // one launch does everything where there are rows and heads enough to fill the card, or little to move
+    const bool all = heads >= 128 || (max_moves + p.recent) * p.units <= 8192;
+#define MM_SELECT(NW_, R_) do { if (all) hipLaunchKernelGGL((evict_select_k<NW_, R_, U, true>), grid, dim3(NW_ * 64), 0, st, p); \
+                                else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
+    if (cap <= 1024) MM_SELECT(4, 4);
+    else if (cap <= 8192) MM_SELECT(16, 8);
+    else if (cap <= 32768) MM_SELECT(16, 32);
+    else if (cap <= 65536) MM_SELECT(16, 64);
+    else MM_SELECT(16, 0);
+#undef MM_SELECT
+    if (all) return;
+    auto split = [&](int64_t items) {                                          // workgroups per (row, KV head): four pieces a thread, 4096 workgroups in all
+        const int64_t w = cdiv(items, 1024), most = cdiv(4096, heads);
+        return (unsigned)(w < 1 ? 1 : w < most ? w : most);
+    };
+    if (max_moves) hipLaunchKernelGGL(evict_moves_k<U>, dim3(grid.x, grid.y, split(max_moves * p.units)), dim3(256), 0, st, p);
+    if (p.recent) hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, split((int64_t)p.recent * p.units)), dim3(256), 0, st, p);
+}
+
 extern "C" int mm_paged_evict(void* kpool, void* vpool, float* weights, const int32_t* page_table, int32_t* lengths, int32_t* kept, int64_t B,
                               int64_t Hkv, int64_t d, int64_t page, int64_t n_pages, int64_t width, int64_t ld_table, int64_t budget,
                               int64_t recent, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
@@ -94,15 +287,20 @@ extern "C" int mm_paged_evict(void* kpool, void* vpool, float* weights, const in
              (long long)budget, (long long)recent);
     if (B == 0) return MM_OK;
     MM_CHECK(weights && lengths && kept && workspace, "paged_evict: null pointer");
+    MM_CHECK(((uintptr_t)weights % 16) == 0, "paged_evict: weights must be 16-byte aligned");
     MM_CHECK(workspace_bytes >= mm_paged_evict_workspace(B, Hkv, page, width, budget, recent), "paged_evict: workspace too small");
+    const int64_t bytes = d * (dtype == MM_BF16 ? 2 : 4), room = evict_room(page, width, budget, recent);
+    const int piece = bytes % 16 == 0 ? 16 : 8;
+    MM_CHECK((room + recent) * (bytes / piece) < (1LL << 31), "paged_evict: too many slots for one call");
     EvictP p{};
-    p.kpool = kpool; p.vpool = vpool; p.w = weights; p.lengths = lengths; p.kept = kept;
+    p.kpool = (char*)kpool; p.vpool = (char*)vpool; p.w = weights; p.lengths = lengths; p.kept = kept;
     p.map = {page_table, (long)ld_table, (int)width, paged_shift(page), (int)n_pages, (int)Hkv};
-    p.keys = (unsigned*)workspace; p.d = (int)d; p.es = dtype == MM_BF16 ? 2 : 4; p.budget = (int)budget; p.recent = (int)recent;
+    p.ws = (int*)workspace; p.room = (int)room; p.units = (int)(bytes / piece); p.budget = (int)budget; p.recent = (int)recent; p.B = (int)B;
     hipStream_t st = (hipStream_t)stream;
-    hipLaunchKernelGGL(paged_evict_k, dim3((unsigned)B, (unsigned)Hkv), dim3(256), 0, st, p);
+    if (piece == 16) evict_launch<mm_u4_t>(p, page * width, room, st);
+    else evict_launch<mm_u2_t>(p, page * width, room, st);
     MM_LAUNCH_CHECK();
-    hipLaunchKernelGGL(paged_lengths_k, dim3((unsigned)cdiv(B, 256)), dim3(256), 0, st, lengths, (int)B, (int)budget, (int)(width * page));
+    hipLaunchKernelGGL(evict_lengths_k, dim3((unsigned)cdiv(B, 256)), dim3(256), 0, st, p);
     MM_LAUNCH_CHECK();
     return MM_OK;
 }
