@@ -442,34 +442,45 @@ __device__ __forceinline__ int paged_cover(const PagedP& p, int b) {
     const int len = p.lengths[b], cap = p.map.capacity();
     return len < 0 ? 0 : min(min(len, cap) + (p.kn ? 1 : 0), cap);
 }
+// Final maximum and 1 / sum of a head over its splits, by one wave (lanes take the splits in turn): every lane gets them.
+__device__ __forceinline__ void paged_final(const PagedP& p, long bh, int ns, float& base, float& inv) {
+    const int lane = threadIdx.x & 63;
+    const float2* st = p.stat + bh * p.nsplit;
+    float M = -INFINITY, L = 0.f;
+    if (!p.stable) {
+        for (int s = lane; s < ns; s += 64) M = fmaxf(M, st[s].x);
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) M = fmaxf(M, __shfl_xor(M, o));
+    }
+    base = p.stable || M == -INFINITY ? 0.f : M;
+    for (int s = lane; s < ns; s += 64) { const float2 e = st[s]; L = fmaf(e.y, p.stable ? 1.f : __builtin_amdgcn_exp2f(e.x - base), L); }
+    L = wave_sum(L);
+    inv = p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
+}
 // Workgroups below `joins`: one (row, head): the splits' outputs, 256 / (d / 4) of them at a time, d / 4 lanes of 16 bytes each.
 // The others: 1024 slots of one (row, KV head): p = exp2(x - max) / sum (| s(x) / sum) of the group's heads, added to the slots' weights.
 template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const PagedP p, int joins, int wchunks) {
     __shared__ __attribute__((aligned(16))) float red[256 * 4];
-    __shared__ float red_l[256];
-    const int tid = threadIdx.x;
+    __shared__ float hb[64], hi[64];
+    const int tid = threadIdx.x, wave = tid >> 6;
     if ((int)blockIdx.x < joins) {
         const int bh = blockIdx.x, b = bh / p.H, cols = p.d >> 2, per = 256 / cols;
         const int c = tid % cols, gr = tid / cols;
         const int ns = (paged_cover(p, b) + p.chunk - 1) / p.chunk;
+        float base, inv;
+        paged_final(p, bh, ns, base, inv);
         const float2* st = p.stat + (long)bh * p.nsplit;
-        float M = -INFINITY;
-        if (!p.stable) for (int s = 0; s < ns; s++) M = fmaxf(M, st[s].x);
-        const float base = p.stable || M == -INFINITY ? 0.f : M;
+        const float* part = p.part + (long)bh * p.nsplit * p.d + c * 4;
         f32x4_t a = {0.f, 0.f, 0.f, 0.f};
-        float L = 0.f;
-        if (gr < per)
-            for (int s = gr; s < ns; s += per) {
-                const float f = p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base);
-                L = fmaf(st[s].y, f, L);
-                a += *reinterpret_cast<const f32x4_t*>(p.part + ((long)bh * p.nsplit + s) * p.d + c * 4) * f;
-            }
+        if (gr < per) {
+#pragma unroll 4
+            for (int s = gr; s < ns; s += per)
+                a += *reinterpret_cast<const f32x4_t*>(part + (long)s * p.d) * (p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base));
+        }
         *reinterpret_cast<f32x4_t*>(red + tid * 4) = a;
-        red_l[tid] = L;
         __syncthreads();
         if (gr == 0) {
-            for (int k = 1; k < per; k++) { a += *reinterpret_cast<f32x4_t*>(red + (k * cols + c) * 4); L += red_l[k * cols + c]; }
-            const float inv = p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
+            for (int k = 1; k < per; k++) a += *reinterpret_cast<f32x4_t*>(red + (k * cols + c) * 4);
             const float r[4] = {a[0] * inv, a[1] * inv, a[2] * inv, a[3] * inv};
             VecIO<T, 4>::store((T*)p.o + (long)bh * p.d + c * 4, r);
         }
@@ -480,28 +491,36 @@ template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const 
     if (s0 >= n) return;
     const int ns = (n + p.chunk - 1) / p.chunk, cap = p.map.capacity();
     const int slot = s0 + tid * 4;
-    f32x4_t add = {0.f, 0.f, 0.f, 0.f};
-    for (int h = 0; h < p.G; h++) {
-        const long bh = (long)b * p.H + hk * p.G + h;
-        const float2* st = p.stat + bh * p.nsplit;
-        float M = -INFINITY, L = 0.f;
-        if (!p.stable) for (int s = 0; s < ns; s++) M = fmaxf(M, st[s].x);
-        const float base = p.stable || M == -INFINITY ? 0.f : M;
-        for (int s = 0; s < ns; s++) L = fmaf(st[s].y, p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base), L);
-        const float inv = p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
-        if (slot < n) {
-            const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.sc + bh * cap + slot);
-#pragma unroll
-            for (int i = 0; i < 4; i++) add[i] += (p.stable ? stable_s(x[i]) : __builtin_amdgcn_exp2f(x[i] - base)) * inv;
+    const long row = slot < n ? p.map.row(b, hk, slot) : -1;                            // four slots of one page (page >= 4)
+    f32x4_t old = {0.f, 0.f, 0.f, 0.f}, add = old;
+    if (row >= 0) old = *reinterpret_cast<const f32x4_t*>(p.w + row);
+    for (int g0 = 0; g0 < p.G; g0 += 64) {
+        const int ng = min(64, p.G - g0);
+        const long bh = (long)b * p.H + hk * p.G + g0;
+        if (g0) __syncthreads();
+        for (int h = wave; h < ng; h += 4) {
+            float base, inv;
+            paged_final(p, bh + h, ns, base, inv);
+            if ((tid & 63) == 0) { hb[h] = base; hi[h] = inv; }
         }
+        __syncthreads();
+        if (row >= 0)
+#pragma unroll 4
+            for (int h = 0; h < ng; h++) {
+                const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.sc + (bh + h) * cap + slot);
+#pragma unroll
+                for (int i = 0; i < 4; i++) add[i] += (p.stable ? stable_s(x[i]) : __builtin_amdgcn_exp2f(x[i] - hb[h])) * hi[h];
+            }
     }
-    if (slot >= n) return;
-    const long row = p.map.row(b, hk, slot);                                            // four slots of one page (page >= 4)
     if (row < 0) return;
     const int len = p.lengths[b];
+    if (slot + 4 <= n && !(p.kn && slot + 4 > len)) {
+        *reinterpret_cast<f32x4_t*>(p.w + row) = old + add;
+    } else {
 #pragma unroll
-    for (int i = 0; i < 4; i++)
-        if (slot + i < n) p.w[row + i] = p.kn && slot + i == len ? add[i] : p.w[row + i] + add[i];
+        for (int i = 0; i < 4; i++)
+            if (slot + i < n) p.w[row + i] = p.kn && slot + i == len ? add[i] : old[i] + add[i];
+    }
 }
 
 // How a cache of `cap` slots is split.  A workgroup takes whole rounds of 128 slots.
@@ -546,7 +565,7 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
              "paged_decode_attn: bad rot/tables");
     MM_CHECK(a->ld_q >= 0 && a->ld_k >= 0 && a->ld_v >= 0, "paged_decode_attn: negative row stride");
     MM_CHECK(a->mode == MM_ATTN_SOFTMAX || a->mode == MM_ATTN_STABLEMAX, "paged_decode_attn: bad mode %d", a->mode);
-    MM_CHECK(((uintptr_t)a->o % 16) == 0, "paged_decode_attn: o must be 16-byte aligned");
+    MM_CHECK((((uintptr_t)a->o | (uintptr_t)a->weights) % 16) == 0, "paged_decode_attn: o and weights must be 16-byte aligned");
     const PagedPlan r = paged_plan(a);
     const size_t need = r.part + r.stat + r.sc;
     MM_CHECK(need == 0 || (a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0), "paged_decode_attn: workspace too small or not 16-byte aligned");
@@ -595,15 +614,15 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
 }
 
 // ------------------------------------------------------------------------------------------------ runs of keys and values
-// A copy: keys and values are read once and written once (4 bytes moved per bf16 value and tensor), which HBM bounds.  A lane moves VE
-// consecutive values of one head of one token; for a rotated key it also reads the partner values (the other half: in the same
-// row, so from the cache that has just fetched it), which spares an exchange between lanes.  VE = 8 (bf16) or 4 (f32) where head_dim,
-// rot / 2 and the strides are multiples of it and the rows are aligned, else 1.
+// A copy: keys and values are read once and written once, which HBM bounds.  A lane moves VE consecutive values of one head of one token;
+// for a rotated key it also reads the partner values (the other half: in the same row, so from the cache that has just fetched it),
+// which spares an exchange between lanes.  VE = 8 (bf16) or 4 (f32) where head_dim and the strides are multiples of it and the rows are
+// aligned, else 1; PV: the halves are multiples of VE too, so that partners are loaded as wide.
 struct FillP {
     const void* k; const void* v; void* kpool; void* vpool; float* w; const int* start; const int* counts; const int* positions;
     const float* cos_t; const float* sin_t; PagedMap map; int S, Hkv, d, rot, n_pos; long ld_k, bs_k, ld_v, bs_v;
 };
-template <typename T, int VE> __global__ __launch_bounds__(256) void paged_fill_k(const FillP p) {
+template <typename T, int VE, bool PV> __global__ __launch_bounds__(256) void paged_fill_k(const FillP p) {
     const int b = blockIdx.y;
     const unsigned pieces = (unsigned)p.d / VE, per = pieces * (unsigned)p.Hkv;
     const unsigned idx = blockIdx.x * 256u + threadIdx.x;                // over [S][Hkv][d / VE]; fits (checked by the launch)
@@ -619,16 +638,27 @@ template <typename T, int VE> __global__ __launch_bounds__(256) void paged_fill_
     VecIO<T, VE>::load(v + c, y);
     const int half = p.rot >> 1;
     if (c < p.rot) {
-        const bool low = c < half;
-        const int i = low ? c : c - half;
         const long pos = p.positions ? (long)p.positions[b] + s : (long)st + s;
-        const long t = min(max(pos, 0L), (long)p.n_pos - 1) * half + i;
-        float o[VE];
-        VecIO<T, VE>::load(k + (low ? c + half : i), o);
+        const long t = min(max(pos, 0L), (long)p.n_pos - 1) * half;
+        if constexpr (PV) {
+            const bool low = c < half;
+            const int i = low ? c : c - half;
+            float o[VE];
+            VecIO<T, VE>::load(k + (low ? c + half : i), o);
 #pragma unroll
-        for (int e = 0; e < VE; e++) {
-            const float cs = p.cos_t[t + e], sn = p.sin_t[t + e];
-            x[e] = low ? fmaf(x[e], cs, -(o[e] * sn)) : fmaf(x[e], cs, o[e] * sn);
+            for (int e = 0; e < VE; e++) {
+                const float cs = p.cos_t[t + i + e], sn = p.sin_t[t + i + e];
+                x[e] = low ? fmaf(x[e], cs, -(o[e] * sn)) : fmaf(x[e], cs, o[e] * sn);
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < VE; e++)
+                if (c + e < p.rot) {
+                    const bool low = c + e < half;
+                    const int i = low ? c + e : c + e - half;
+                    const float o = to_f(k[low ? c + e + half : i]), cs = p.cos_t[t + i], sn = p.sin_t[t + i];
+                    x[e] = low ? fmaf(x[e], cs, -(o * sn)) : fmaf(x[e], cs, o * sn);
+                }
         }
     }
     const long row = p.map.row(b, h, st + s);
@@ -654,19 +684,19 @@ extern "C" int mm_paged_cache_fill(const mm_paged_fill_args* a, void* stream) {
     p.S = (int)a->S; p.Hkv = (int)a->Hkv; p.d = (int)a->d; p.rot = (int)a->rot; p.n_pos = a->rot ? (int)a->n_pos : 1;
     p.ld_k = a->ld_k; p.bs_k = a->bs_k; p.ld_v = a->ld_v; p.bs_v = a->bs_v;
     const int VE = a->dtype == MM_BF16 ? 8 : 4;
-    const int64_t all = a->d | a->rot / 2 | a->ld_k | a->bs_k | a->ld_v | a->bs_v;
-    const bool wide = all % VE == 0 && (((uintptr_t)a->k | (uintptr_t)a->v) % 16) == 0;
+    const int64_t all = a->d | a->ld_k | a->bs_k | a->ld_v | a->bs_v;
+    const bool wide = all % VE == 0 && (((uintptr_t)a->k | (uintptr_t)a->v) % 16) == 0, pv = a->rot / 2 % VE == 0;
     const int64_t items = a->S * a->Hkv * (a->d / (wide ? VE : 1));
     MM_CHECK(items < (1LL << 31), "paged_cache_fill: too many tokens for one call");
     const dim3 grid((unsigned)cdiv(items, 256), (unsigned)a->B);
     hipStream_t st = (hipStream_t)stream;
+#define MM_FILL(T_, VE_, PV_) hipLaunchKernelGGL((paged_fill_k<T_, VE_, PV_>), grid, dim3(256), 0, st, p)
     if (a->dtype == MM_BF16) {
-        if (wide) hipLaunchKernelGGL((paged_fill_k<bf16, 8>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((paged_fill_k<bf16, 1>), grid, dim3(256), 0, st, p);
+        if (wide && pv) MM_FILL(bf16, 8, true); else if (wide) MM_FILL(bf16, 8, false); else MM_FILL(bf16, 1, true);
     } else {
-        if (wide) hipLaunchKernelGGL((paged_fill_k<float, 4>), grid, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((paged_fill_k<float, 1>), grid, dim3(256), 0, st, p);
+        if (wide && pv) MM_FILL(float, 4, true); else if (wide) MM_FILL(float, 4, false); else MM_FILL(float, 1, true);
     }
+#undef MM_FILL
     MM_LAUNCH_CHECK();
     return MM_OK;
 }

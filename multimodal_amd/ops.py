@@ -355,76 +355,103 @@ def decode_attn(q: Tensor, k_new: Tensor, v_new: Tensor, kcache: Tensor, vcache:
 
 
 # --------------------------------------------------------------------------- paged key-value cache
-class _OnDevice:
-    """Makes the tensors' device the current one around a launch (nothing to do where it already is)."""
-
-    def __init__(self, dev):
-        self.guard = None if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+# A serving step issues these calls once per layer and token, and a small one runs for less time than a call's checks once took (12-17 us of
+# Python for 3-8 us of kernel).  So each call asks one cheap question of all its arguments (device numbers, identical dtypes, shapes), and only
+# where the answer is no does a second function look for the reason and name it.
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
+_PAGE_SIZES = frozenset((4, 8, 16, 32, 64, 128, 256, 512, 1024))
+_CODES = {torch.float32: L.MM_F32, torch.bfloat16: L.MM_BF16}
 
 
-def _inference_only(who: str, *tensors: Optional[Tensor]) -> None:
+def _launch(fn, what: str, dev: int, *args) -> None:
+    """Calls a C entry point with the tensors' device current, its last argument that device's current stream."""
+    if dev == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
+    if rc or L._TRACE:
+        L.check(rc, what)
+
+
+def _refuse_grad(who: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError(f"{who}: has no backward pass; call it under torch.no_grad()")
 
 
-def _ids(t: Optional[Tensor], name: str, B: int, dev) -> Optional[Tensor]:
-    """An int32 vector with one element per row."""
-    if t is None:
-        return None
-    _chk(t, name, torch.int32)
-    if t.shape != (B,) or t.device != dev:
-        raise RuntimeError(f"{name}: expected an int32 tensor [{B}] on {dev}, got {tuple(t.shape)} on {t.device}")
-    return t
+def _refuse_ids(who: str, B: int, dev: int, **named: Optional[Tensor]) -> None:
+    for name, t in named.items():
+        if t is None and name == "lengths":
+            raise RuntimeError(f"{who}: lengths are needed")
+        if t is not None:
+            _chk(t, f"{who}: {name}", torch.int32)
+            if t.shape != (B,) or t.get_device() != dev:
+                raise RuntimeError(f"{who}: {name} must be an int32 tensor [{B}] on cuda:{dev}, got {tuple(t.shape)} on {t.device}")
 
 
-def _paged_geom(who: str, kpool: Tensor, vpool: Tensor, page_table: Tensor, weights: Optional[Tensor]):
-    """Checks a paged cache and returns (B, Hkv, d, page, n_pages, width)."""
+def _refuse_rows(who: str, like: Tensor, **named) -> None:
+    """named: name=(tensor, shape)"""
+    for name, (t, shape) in named.items():
+        if not t.is_cuda or tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device \
+                or (t.shape[-1] > 1 and t.stride(-1) != 1):
+            raise RuntimeError(f"{who}: {name}: expected {tuple(shape)} {like.dtype} with unit inner stride on {like.device}, got "
+                               f"{tuple(t.shape)} {t.dtype} on {t.device}")
+
+
+def _refuse_cache(who: str, kpool: Tensor, vpool: Tensor, page_table: Tensor, weights: Optional[Tensor]) -> None:
     _chk(kpool, f"{who}: kpool"); _chk(vpool, f"{who}: vpool", kpool.dtype)
     L.dtype_code(kpool)
     if kpool.dim() != 4 or vpool.shape != kpool.shape or vpool.device != kpool.device or vpool.data_ptr() == kpool.data_ptr():
         raise RuntimeError(f"{who}: kpool and vpool must be two tensors [pages, KV heads, page, head_dim] on one device")
     n_pages, Hkv, page, d = kpool.shape
-    if d % 4 or not 0 < d <= 512 or page not in (4, 8, 16, 32, 64, 128, 256, 512, 1024) or not n_pages or not Hkv:
+    if d % 4 or not 0 < d <= 512 or page not in _PAGE_SIZES or not n_pages or not Hkv:
         raise RuntimeError(f"{who}: pages of {page} slots (a power of two, 4 to 1024), head_dim {d} (a multiple of 4, at most 512)")
     if not page_table.is_cuda or page_table.dtype != torch.int32 or page_table.dim() != 2 or page_table.device != kpool.device \
-            or (page_table.shape[1] > 1 and page_table.stride(1) != 1) or page_table.shape[1] == 0:
+            or page_table.shape[1] == 0 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
         raise RuntimeError(f"{who}: page_table must be an int32 GPU tensor [B, pages per row] with unit inner stride on the pools' device")
     if weights is not None:
         _chk(weights, f"{who}: weights", torch.float32)
         if weights.shape != kpool.shape[:3] or weights.device != kpool.device:
             raise RuntimeError(f"{who}: weights must be float32 [pages, KV heads, page] on the pools' device")
-    return page_table.shape[0], Hkv, d, page, n_pages, page_table.shape[1]
 
 
-def _rope_args(who: str, rot: int, d: int, cos_t: Optional[Tensor], sin_t: Optional[Tensor], dev) -> int:
-    """Checks the rotary tables; returns the positions they hold."""
+def _cache_geom(who: str, kpool: Tensor, vpool: Tensor, page_table: Tensor, weights: Optional[Tensor]):
+    """Checks a paged cache: (device number, dtype code, B, n_pages, Hkv, page, d, width, ld_table)."""
+    dev, dt, shape = kpool.get_device(), kpool.dtype, kpool.shape
+    code = _CODES.get(dt)
+    if code is not None and dev >= 0 and len(shape) == 4 and page_table.dim() == 2:
+        n_pages, Hkv, page, d = shape
+        B, width = page_table.shape
+        ld, inner = page_table.stride()
+        if (vpool.dtype is dt and vpool.shape == shape and vpool.get_device() == dev and kpool.is_contiguous() and vpool.is_contiguous()
+                and page in _PAGE_SIZES and d % 4 == 0 and 0 < d <= 512 and n_pages and Hkv and page_table.dtype is torch.int32
+                and page_table.get_device() == dev and width and (inner == 1 or width == 1) and vpool.data_ptr() != kpool.data_ptr()
+                and (weights is None or (weights.dtype is torch.float32 and weights.shape == shape[:3] and weights.get_device() == dev
+                                         and weights.is_contiguous()))):
+            return dev, code, B, n_pages, Hkv, page, d, width, ld
+    _refuse_cache(who, kpool, vpool, page_table, weights)
+    raise RuntimeError(f"{who}: not a paged cache")
+
+
+def _ids_ok(t: Optional[Tensor], B: int, dev: int) -> bool:
+    return t is None or (t.dtype is torch.int32 and t.get_device() == dev and t.shape == (B,) and (t.stride(0) == 1 or B < 2))
+
+
+def _rope_args(who: str, rot: int, d: int, cos_t: Optional[Tensor], sin_t: Optional[Tensor], dev: int):
+    """Checks the rotary tables: (address of cos, address of sin, positions they hold)."""
+    if rot == 0:
+        return None, None, 0
     if rot < 0 or rot % 2 or rot > d:
         raise RuntimeError(f"{who}: rot={rot} must be even and at most head_dim ({d})")
-    if rot == 0:
-        return 0
     if cos_t is None or sin_t is None:
         raise RuntimeError(f"{who}: rot={rot} needs the cos and sin tables")
-    for t, nm in ((cos_t, "cos_t"), (sin_t, "sin_t")):
-        _f32(t, f"{who}: {nm}")
-        if t.dim() != 2 or t.shape[1] != rot // 2 or t.shape != cos_t.shape or t.shape[0] == 0 or t.device != dev:
-            raise RuntimeError(f"{who}: {nm} must be float32 [positions, {rot // 2}] on the pools' device")
-    return cos_t.shape[0]
-
-
-def _rows(t: Tensor, name: str, shape, like: Tensor) -> Tensor:
-    if not t.is_cuda or tuple(t.shape) != tuple(shape) or t.dtype != like.dtype or t.device != like.device \
-            or (t.shape[-1] > 1 and t.stride(-1) != 1):
-        raise RuntimeError(f"{name}: expected {tuple(shape)} {like.dtype} with unit inner stride on {like.device}, got {tuple(t.shape)} "
-                           f"{t.dtype} on {t.device}")
-    return t
+    shape = cos_t.shape
+    if not (len(shape) == 2 and shape[1] == rot // 2 and shape[0] and sin_t.shape == shape and cos_t.dtype is torch.float32
+            and sin_t.dtype is torch.float32 and cos_t.get_device() == dev and sin_t.get_device() == dev and cos_t.is_contiguous()
+            and sin_t.is_contiguous()):
+        raise RuntimeError(f"{who}: cos_t and sin_t must be contiguous float32 [positions, {rot // 2}] on cuda:{dev}")
+    return cos_t.data_ptr(), sin_t.data_ptr(), shape[0]
 
 
 def paged_decode_attn(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor], kpool: Tensor, vpool: Tensor, page_table: Tensor,
@@ -440,29 +467,40 @@ def paged_decode_attn(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor
     draws (paged_evict goes by it).  A row with lengths < 0 sits out; a row without a slot, and one that sits out, gets zeros.  A token
     whose page the table does not hold is neither stored nor attended.  Pages written by a call belong to one row.  Returns o [B, H*d]."""
     who = "paged_decode_attn"
-    _inference_only(who, q, k_new, v_new, kpool, vpool, weights)
-    B, Hkv, d, page, n_pages, width = _paged_geom(who, kpool, vpool, page_table, weights)
+    dev, code, B, n_pages, Hkv, page, d, width, ld_table = _cache_geom(who, kpool, vpool, page_table, weights)
     if H <= 0 or H % Hkv:
         raise RuntimeError(f"{who}: {H} query heads over {Hkv} KV heads")
     if (k_new is None) != (v_new is None):
         raise RuntimeError(f"{who}: k_new and v_new come together")
-    _rows(q, f"{who}: q", (B, H * d), kpool)
-    if k_new is not None:
-        _rows(k_new, f"{who}: k_new", (B, Hkv * d), kpool); _rows(v_new, f"{who}: v_new", (B, Hkv * d), kpool)
-    dev = kpool.device
-    _ids(lengths, f"{who}: lengths", B, dev); _ids(positions, f"{who}: positions", B, dev)
-    o = torch.empty((B, H * d), dtype=q.dtype, device=dev)
-    a = L.PagedAttnArgs(
-        q.data_ptr(), L.ptr(k_new), L.ptr(v_new), kpool.data_ptr(), vpool.data_ptr(), o.data_ptr(), L.ptr(weights), page_table.data_ptr(),
-        lengths.data_ptr(), L.ptr(positions), L.ptr(cos_t) if rot else None, L.ptr(sin_t) if rot else None, B, H, Hkv, d, rot, page, n_pages,
-        width, page_table.stride(0), q.stride(0), 0 if k_new is None else k_new.stride(0), 0 if v_new is None else v_new.stride(0),
-        _rope_args(who, rot, d, cos_t, sin_t, dev), int(stablemax), L.dtype_code(kpool))
-    nbytes = L.lib().mm_paged_decode_attn_workspace(C.byref(a))
-    with _OnDevice(dev):
+    dt, kv = kpool.dtype, (B, Hkv * d)
+    ok = q.dtype is dt and q.get_device() == dev and q.shape == (B, H * d)
+    kp = vp = None
+    ld_k = ld_v = 0
+    if k_new is not None and ok:
+        ok = k_new.dtype is dt and v_new.dtype is dt and k_new.get_device() == dev and v_new.get_device() == dev and k_new.shape == kv \
+            and v_new.shape == kv
+        if ok:
+            kp, vp, (ld_k, ik), (ld_v, iv) = k_new.data_ptr(), v_new.data_ptr(), k_new.stride(), v_new.stride()
+            ok = ik == 1 and iv == 1
+    if not (ok and q.stride(1) == 1):
+        _refuse_rows(who, kpool, q=(q, (B, H * d)))
+        _refuse_rows(who, kpool, k_new=(k_new, kv), v_new=(v_new, kv))
+    if not (_ids_ok(lengths, B, dev) and _ids_ok(positions, B, dev) and lengths is not None):
+        _refuse_ids(who, B, dev, lengths=lengths, positions=positions)
+    if torch.is_grad_enabled():
+        _refuse_grad(who, q, k_new, v_new, kpool, vpool, weights)
+    cp, sp, n_pos = _rope_args(who, rot, d, cos_t, sin_t, dev)
+    o = q.new_empty((B, H * d))
+    a = L.PagedAttnArgs(q.data_ptr(), kp, vp, kpool.data_ptr(), vpool.data_ptr(), o.data_ptr(), None if weights is None else weights.data_ptr(),
+                        page_table.data_ptr(), lengths.data_ptr(), None if positions is None else positions.data_ptr(), cp, sp, B, H, Hkv, d,
+                        rot, page, n_pages, width, ld_table, q.stride(0), ld_k, ld_v, n_pos, 1 if stablemax else 0, code)
+    lib, ref = L.lib(), C.byref(a)
+    nbytes = lib.mm_paged_decode_attn_workspace(ref)
+    if nbytes:
         # a buffer of its own per call: calls on two streams, and graphs captured on one stream and replayed beside each other, share none
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        a.workspace, a.workspace_bytes = L.ptr(ws), nbytes
-        L.check(L.lib().mm_paged_decode_attn(C.byref(a), L.cur_stream()), "mm_paged_decode_attn")
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), nbytes
+    _launch(lib.mm_paged_decode_attn, "mm_paged_decode_attn", dev, ref)
     return o
 
 
@@ -474,21 +512,28 @@ def paged_cache_fill(k: Tensor, v: Tensor, kpool: Tensor, vpool: Tensor, page_ta
     [B].  Rows with start < 0 store nothing; tokens whose page the table does not hold are left out; the rest of a padded batch is not
     read.  weights: set to 0 for the stored slots."""
     who = "paged_cache_fill"
-    _inference_only(who, k, v, kpool, vpool, weights)
-    B, Hkv, d, page, n_pages, width = _paged_geom(who, kpool, vpool, page_table, weights)
+    dev, code, B, n_pages, Hkv, page, d, width, ld_table = _cache_geom(who, kpool, vpool, page_table, weights)
     if k.dim() != 3:
         raise RuntimeError(f"{who}: k must be [B, S, KV heads * head_dim]")
-    S = k.shape[1]
-    _rows(k, f"{who}: k", (B, S, Hkv * d), kpool); _rows(v, f"{who}: v", (B, S, Hkv * d), kpool)
-    dev = kpool.device
-    _ids(start, f"{who}: start", B, dev); _ids(counts, f"{who}: counts", B, dev); _ids(positions, f"{who}: positions", B, dev)
-    a = L.PagedFillArgs(
-        k.data_ptr(), v.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), L.ptr(weights), page_table.data_ptr(), L.ptr(start), L.ptr(counts),
-        L.ptr(positions), L.ptr(cos_t) if rot else None, L.ptr(sin_t) if rot else None, B, S, Hkv, d, rot, page, n_pages, width,
-        page_table.stride(0), k.stride(1), k.stride(0), v.stride(1), v.stride(0), _rope_args(who, rot, d, cos_t, sin_t, dev),
-        L.dtype_code(kpool))
-    with _OnDevice(dev):
-        L.check(L.lib().mm_paged_cache_fill(C.byref(a), L.cur_stream()), "mm_paged_cache_fill")
+    dt, S = kpool.dtype, k.shape[1]
+    shape = (B, S, Hkv * d)
+    ok = k.dtype is dt and v.dtype is dt and k.get_device() == dev and v.get_device() == dev and k.shape == shape and v.shape == shape
+    if ok:
+        (bs_k, ld_k, ik), (bs_v, ld_v, iv) = k.stride(), v.stride()
+        ok = ik == 1 and iv == 1
+    if not ok:
+        _refuse_rows(who, kpool, k=(k, shape), v=(v, shape))
+        (bs_k, ld_k, ik), (bs_v, ld_v, iv) = k.stride(), v.stride()
+    if not (_ids_ok(start, B, dev) and _ids_ok(counts, B, dev) and _ids_ok(positions, B, dev)):
+        _refuse_ids(who, B, dev, start=start, counts=counts, positions=positions)
+    if torch.is_grad_enabled():
+        _refuse_grad(who, k, v, kpool, vpool, weights)
+    cp, sp, n_pos = _rope_args(who, rot, d, cos_t, sin_t, dev)
+    a = L.PagedFillArgs(k.data_ptr(), v.data_ptr(), kpool.data_ptr(), vpool.data_ptr(), None if weights is None else weights.data_ptr(),
+                        page_table.data_ptr(), None if start is None else start.data_ptr(), None if counts is None else counts.data_ptr(),
+                        None if positions is None else positions.data_ptr(), cp, sp, B, S, Hkv, d, rot, page, n_pages, width, ld_table, ld_k,
+                        bs_k, ld_v, bs_v, n_pos, code)
+    _launch(L.lib().mm_paged_cache_fill, "mm_paged_cache_fill", dev, C.byref(a))
 
 
 def paged_evict(kpool: Tensor, vpool: Tensor, weights: Tensor, page_table: Tensor, lengths: Tensor, budget: int, recent: int) -> Tensor:
@@ -500,19 +545,20 @@ def paged_evict(kpool: Tensor, vpool: Tensor, weights: Tensor, page_table: Tenso
     who = "paged_evict"
     if weights is None:
         raise RuntimeError(f"{who}: weights are what it goes by")
-    _inference_only(who, kpool, vpool, weights)
-    B, Hkv, d, page, n_pages, width = _paged_geom(who, kpool, vpool, page_table, weights)
+    dev, code, B, n_pages, Hkv, page, d, width, ld_table = _cache_geom(who, kpool, vpool, page_table, weights)
     if not 0 < budget < 1 << 30 or not 0 <= recent <= budget:
         raise RuntimeError(f"{who}: budget={budget} recent={recent}: 0 <= recent <= budget and budget > 0")
-    dev = kpool.device
-    _ids(lengths, f"{who}: lengths", B, dev)
-    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
-    nbytes = L.lib().mm_paged_evict_workspace(B, Hkv, page, width, budget, recent)
-    with _OnDevice(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        L.check(L.lib().mm_paged_evict(kpool.data_ptr(), vpool.data_ptr(), weights.data_ptr(), page_table.data_ptr(), lengths.data_ptr(),
-                                       kept.data_ptr(), B, Hkv, d, page, n_pages, width, page_table.stride(0), budget, recent,
-                                       L.dtype_code(kpool), L.ptr(ws), nbytes, L.cur_stream()), "mm_paged_evict")
+    if not (_ids_ok(lengths, B, dev) and lengths is not None):
+        _refuse_ids(who, B, dev, lengths=lengths)
+    if torch.is_grad_enabled():
+        _refuse_grad(who, kpool, vpool, weights)
+    kept = lengths.new_empty((B, Hkv, budget))
+    lib = L.lib()
+    nbytes = lib.mm_paged_evict_workspace(B, Hkv, page, width, budget, recent)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=lengths.device) if nbytes else None      # its own: as in paged_decode_attn
+    _launch(lib.mm_paged_evict, "mm_paged_evict", dev, kpool.data_ptr(), vpool.data_ptr(), weights.data_ptr(), page_table.data_ptr(),
+            lengths.data_ptr(), kept.data_ptr(), B, Hkv, d, page, n_pages, width, ld_table, budget, recent, code,
+            None if ws is None else ws.data_ptr(), nbytes)
     return kept
 
 
@@ -526,28 +572,35 @@ def verify_drafts(drafts: Tensor, p: Tensor, u: Tensor, q: Optional[Tensor] = No
     counts int32 [B]: drafts a row really has.  Rows may be strided, the inner stride is 1.  Returns tokens int64 [B, K+1] (accepted
     drafts, the last token, then -1) and the number accepted, int32 [B]."""
     who = "verify_drafts"
-    _inference_only(who, p, q)
-    if drafts.dim() != 2 or p.dim() != 3 or not drafts.is_cuda or drafts.dtype != torch.int64 or drafts.device != p.device \
+    dev = p.get_device()
+    if drafts.dim() != 2 or p.dim() != 3 or dev < 0 or drafts.dtype is not torch.int64 or drafts.get_device() != dev \
             or (drafts.shape[1] > 1 and drafts.stride(1) != 1):
         raise RuntimeError(f"{who}: drafts must be an int64 GPU tensor [B, K] with unit inner stride on the device of p [B, K + 1, V]")
     B, K = drafts.shape
     V = p.shape[2]
-    if p.dtype != torch.float32 or V == 0:
+    f32 = torch.float32
+    if p.dtype is not f32 or V == 0:
         raise TypeError(f"{who}: p must hold float32 probabilities [B, K + 1, V], got {p.dtype} {tuple(p.shape)}")
-    _rows(p, f"{who}: p", (B, K + 1, V), p); _rows(u, f"{who}: u", (B, K + 1), p)
-    if q is not None:
-        _rows(q, f"{who}: q", (B, K, V), p)
-    dev = p.device
-    _ids(counts, f"{who}: counts", B, dev)
-    tokens = torch.empty((B, K + 1), dtype=torch.int64, device=dev)
-    accepted = torch.empty(B, dtype=torch.int32, device=dev)
-    nbytes = L.lib().mm_verify_drafts_workspace(B, V)
-    with _OnDevice(dev):
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        a = L.VerifyArgs(drafts.data_ptr(), p.data_ptr(), L.ptr(q), u.data_ptr(), L.ptr(counts), tokens.data_ptr(), accepted.data_ptr(),
-                         B, K, V, drafts.stride(0), p.stride(0), p.stride(1), 0 if q is None else q.stride(0),
-                         0 if q is None else q.stride(1), u.stride(0), L.ptr(ws), nbytes)
-        L.check(L.lib().mm_verify_drafts(C.byref(a), L.cur_stream()), "mm_verify_drafts")
+    bs_p, ld_p, ip = p.stride()
+    ld_u, iu = u.stride() if u.dim() == 2 else (0, 0)
+    bs_q, ld_q, iq = (0, 0, 1) if q is None else q.stride() if q.dim() == 3 else (0, 0, 0)
+    if not (p.shape == (B, K + 1, V) and ip == 1 and u.dtype is f32 and u.get_device() == dev and u.shape == (B, K + 1) and iu == 1 and iq == 1
+            and (q is None or (q.dtype is f32 and q.get_device() == dev and q.shape == (B, K, V)))):
+        _refuse_rows(who, p, p=(p, (B, K + 1, V)), u=(u, (B, K + 1)))
+        if q is not None:
+            _refuse_rows(who, p, q=(q, (B, K, V)))
+    if not _ids_ok(counts, B, dev):
+        _refuse_ids(who, B, dev, counts=counts)
+    if torch.is_grad_enabled():
+        _refuse_grad(who, p, q)
+    tokens, accepted = drafts.new_empty((B, K + 1)), drafts.new_empty((B,), dtype=torch.int32)
+    lib = L.lib()
+    nbytes = lib.mm_verify_drafts_workspace(B, V)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=p.device) if nbytes else None
+    a = L.VerifyArgs(drafts.data_ptr(), p.data_ptr(), None if q is None else q.data_ptr(), u.data_ptr(),
+                     None if counts is None else counts.data_ptr(), tokens.data_ptr(), accepted.data_ptr(), B, K, V, drafts.stride(0), bs_p, ld_p,
+                     bs_q, ld_q, ld_u, None if ws is None else ws.data_ptr(), nbytes)
+    _launch(lib.mm_verify_drafts, "mm_verify_drafts", dev, C.byref(a))
     return tokens, accepted
 
 
