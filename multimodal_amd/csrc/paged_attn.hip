@@ -27,7 +27,7 @@ struct PagedP {
     const void* q; const void* kn; const void* vn; void* kpool; void* vpool; void* o; float* w; const int* lengths; const int* positions;
     const float* cos_t; const float* sin_t; PagedMap map;
     float* part; float2* stat; float* sc;       // per (row, head, split): unscaled output [d], (max, sum); scores [row][head][capacity]
-    int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, stable; long ld_q, ld_k, ld_v; float scale;
+    int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, units, stable; long ld_q, ld_k, ld_v; float scale;
 };
 
 __device__ __forceinline__ int paged_pos(const int* positions, const int* lengths, bool append, int n_pos, int b) {
@@ -70,19 +70,20 @@ __device__ __forceinline__ void lds_barrier() {
 // VE: columns a lane loads of a V row (16 lanes x VE = one slab), NS: slabs of a head, NT: tiles of 16 slots in a step, AL8: rows are
 // multiples of 8 values (16-byte pieces).  K of the whole step is in registers; of V up to two slabs, the others follow as those are used
 // up (a head of 512 would need 512 registers for its step otherwise).
-template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
+template <typename T, int VE_, int NS_, int NT_, bool AL8, bool ST> struct Step {
     static constexpr bool BF = std::is_same<T, bf16>::value;
     static constexpr int VE = VE_, NS = NS_, NT = NT_, J = 4 * NT, DP = 16 * VE * NS;
     static constexpr int PE = BF ? 8 : 4, CW = 4 * PE, KC = DP / CW;           // values in a lane's piece of K, columns of a matrix instruction
-    static constexpr int QT = BF ? 3 : 1, QFRAG = QT * KC * 64 * 16;           // terms of q, bytes of its fragments in LDS
+    static constexpr int QT = BF ? 3 : 1, QS = DP + PE;                        // terms of q; a head's row in LDS (one piece of padding: no bank conflicts)
     static constexpr int VB = NS < 2 ? NS : 2;
-    static constexpr bool QREG = DP <= 128;                                    // wider heads read the q fragments from LDS every step
-    static_assert(!BF || NT == 2, "the bf16 products take 32 slots");
     typedef typename std::conditional<VE * sizeof(T) == 16, u4_t, u2_t>::type v_t;
+    template <typename V> static __device__ __forceinline__ V read(const T* p) {
+        if constexpr (ST) return __builtin_nontemporal_load(reinterpret_cast<const V*>(p));
+        else return *reinterpret_cast<const V*>(p);
+    }
     typedef __attribute__((ext_vector_type(8))) __bf16 frag_t;
     u4_t k[NT][KC];
     v_t v[VB][J];
-    u4_t q[QREG ? QT : 1][QREG ? KC : 1];
 
     __device__ __forceinline__ void load_k(const T* pool, const long (&row)[NT], int d, int g) {
 #pragma unroll
@@ -92,9 +93,9 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
             for (int c = 0; c < KC; c++) {
                 const int col = c * CW + g * PE;
                 if constexpr (AL8) {
-                    k[t][c] = *reinterpret_cast<const u4_t*>(r + (col < d ? col : 0));
+                    k[t][c] = read<u4_t>(r + (col < d ? col : 0));
                 } else {
-                    const u2_t a = *reinterpret_cast<const u2_t*>(r + (col < d ? col : 0)), b = *reinterpret_cast<const u2_t*>(r + (col + 4 < d ? col + 4 : 0));
+                    const u2_t a = read<u2_t>(r + (col < d ? col : 0)), b = read<u2_t>(r + (col + 4 < d ? col + 4 : 0));
                     k[t][c] = u4_t{a[0], a[1], b[0], b[1]};
                 }
             }
@@ -118,7 +119,7 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
 #pragma unroll
         for (int t = 0; t < NT; t++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) v[s % VB][t * 4 + i] = *reinterpret_cast<const v_t*>(pool + (row[t] + i) * d + cc);
+            for (int i = 0; i < 4; i++) v[s % VB][t * 4 + i] = read<v_t>(pool + (row[t] + i) * d + cc);
     }
     __device__ __forceinline__ void load_v(const T* pool, const long (&row)[NT], int d, int li) {
 #pragma unroll
@@ -134,38 +135,31 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
 #pragma unroll
             for (int c = 0; c < KC; c++) k[0][c] = *reinterpret_cast<const u4_t*>(ks + c * CW + g * PE);
     }
-    // q fragments: value (head, column), in lane (group * 16 + head) of its chunk, as QT terms
-    static __device__ __forceinline__ void put_q(char* lds, int head, int c, float x) {
-        T* f = (T*)lds;
-        const int at = ((c / CW) * 64 + (c / PE % 4) * 16 + head) * PE + c % PE;
-        if constexpr (!BF) { f[at] = x; return; }
+    // value (head, column) of q, as QT terms: rows [term][heads]
+    static __device__ __forceinline__ void put_q(T* lds, int heads, int head, int c, float x) {
+        T* f = lds + head * QS + c;
+        if constexpr (!BF) { *f = x; return; }
         const float least = x == 0.f ? 0.f : copysignf(0x1p-100f, x);
 #pragma unroll
         for (int t = 0; t < QT; t++) {
             const float h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-            f[t * KC * 64 * PE + at] = from_f<T>(t && h == 0.f ? least : h);
+            f[t * heads * QS] = from_f<T>(t && h == 0.f ? least : h);
             x -= h;
         }
     }
-    __device__ __forceinline__ void get_q(const char* lds, int lane) {
-        if constexpr (QREG)
+    // the scores of the step's tiles; q: this lane's head and piece in LDS.  Columns that are not rotated are exact in q's first term.
+    __device__ __forceinline__ void scores(const T* q, int heads, int rot, f32x4_t (&s)[NT]) const {
+        f32x4_t even[NT];                                                      // two chains of sums: a product's result takes several cycles
 #pragma unroll
-            for (int t = 0; t < QT; t++)
-#pragma unroll
-                for (int c = 0; c < KC; c++) q[t][c] = *reinterpret_cast<const u4_t*>(lds + ((t * KC + c) * 64 + lane) * 16);
-    }
-    // the scores of the step's tiles.  Columns that are not rotated are exact in q's first term.
-    __device__ __forceinline__ void scores(const char* lds, int lane, int rot, f32x4_t (&s)[NT]) const {
-#pragma unroll
-        for (int h = 0; h < NT; h++) s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int h = 0; h < NT; h++) { s[h] = f32x4_t{0.f, 0.f, 0.f, 0.f}; even[h] = s[h]; }
+        int z = 0;
+        asm volatile("" : "+v"(z));                                            // read again every step: registers are for the cache's rows
 #pragma unroll
         for (int c = 0; c < KC; c++)
 #pragma unroll
             for (int t = 0; t < QT; t++) {
                 if (t && c * CW >= rot) break;
-                u4_t qf;
-                if constexpr (QREG) qf = q[t][c];
-                else qf = *reinterpret_cast<const u4_t*>(lds + ((t * KC + c) * 64 + lane) * 16);
+                const u4_t qf = *reinterpret_cast<const u4_t*>(q + (t * heads * QS + c * CW) + z);
 #pragma unroll
                 for (int h = 0; h < NT; h++) {
                     if constexpr (BF) {
@@ -173,10 +167,16 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
                     } else {
                         const f32x4_t kf = __builtin_bit_cast(f32x4_t, k[h][c]), qq = __builtin_bit_cast(f32x4_t, qf);
 #pragma unroll
-                        for (int j = 0; j < 4; j++) s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s[h], 0, 0, 0);
+                        for (int j = 0; j < 4; j += 2) {
+                            s[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j], qq[j], s[h], 0, 0, 0);
+                            even[h] = __builtin_amdgcn_mfma_f32_16x16x4f32(kf[j + 1], qq[j + 1], even[h], 0, 0, 0);
+                        }
                     }
                 }
             }
+        if constexpr (!BF)
+#pragma unroll
+            for (int h = 0; h < NT; h++) s[h] += even[h];
     }
     // acc[slab][column][4] += V^T P^T over one slab; slots whose bit is not set have p = 0, and their V must not be inf or NaN
     __device__ __forceinline__ void slab(int s, const float (&p)[J], unsigned ok, f32x4_t (&acc)[NS][VE]) {
@@ -188,24 +188,30 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
         if constexpr (BF) {
             typedef __attribute__((ext_vector_type(2))) float f2_t;
             typedef __attribute__((ext_vector_type(2))) __bf16 b2_t;
-            unsigned hi[4], lo[4];
+            constexpr int W = J / 2;                                           // 32-bit words of an operand: 4 (32 slots) or 2 (16)
+            unsigned hi[W], lo[W];
 #pragma unroll
-            for (int m = 0; m < 4; m++) {
+            for (int m = 0; m < W; m++) {
                 const unsigned a = __float_as_uint(p[2 * m]), b = __float_as_uint(p[2 * m + 1]);
                 hi[m] = __builtin_amdgcn_perm(b, a, 0x07060302u);
                 lo[m] = __builtin_bit_cast(unsigned, __builtin_convertvector((f2_t{fmaxf(p[2 * m] - __uint_as_float(a & 0xffff0000u), 0x1p-100f),
                                                                                   fmaxf(p[2 * m + 1] - __uint_as_float(b & 0xffff0000u), 0x1p-100f)}), b2_t));
             }
-            const frag_t ph = __builtin_bit_cast(frag_t, (u4_t{hi[0], hi[1], hi[2], hi[3]})), pl = __builtin_bit_cast(frag_t, (u4_t{lo[0], lo[1], lo[2], lo[3]}));
 #pragma unroll
             for (int e = 0; e < VE; e++) {
-                unsigned x[4];
+                unsigned x[W];
 #pragma unroll
-                for (int m = 0; m < 4; m++)                                    // two slots' halfwords side by side
+                for (int m = 0; m < W; m++)                                    // two slots' halfwords side by side
                     x[m] = __builtin_amdgcn_perm(w[2 * m + 1][e >> 1], w[2 * m][e >> 1], e & 1 ? 0x07060302u : 0x05040100u);
-                const frag_t a = __builtin_bit_cast(frag_t, (u4_t{x[0], x[1], x[2], x[3]}));
-                acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, ph, acc[s][e], 0, 0, 0);
-                acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, pl, acc[s][e], 0, 0, 0);
+                if constexpr (NT == 2) {
+                    const frag_t a = __builtin_bit_cast(frag_t, (u4_t{x[0], x[1], x[2], x[3]}));
+                    acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(frag_t, (u4_t{hi[0], hi[1], hi[2], hi[3]})), acc[s][e], 0, 0, 0);
+                    acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, __builtin_bit_cast(frag_t, (u4_t{lo[0], lo[1], lo[2], lo[3]})), acc[s][e], 0, 0, 0);
+                } else {
+                    const bf16x4_t a = __builtin_bit_cast(bf16x4_t, (u2_t{x[0], x[1]}));
+                    acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, __builtin_bit_cast(bf16x4_t, (u2_t{hi[0], hi[1]})), acc[s][e], 0, 0, 0);
+                    acc[s][e] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(a, __builtin_bit_cast(bf16x4_t, (u2_t{lo[0], lo[1]})), acc[s][e], 0, 0, 0);
+                }
             }
         } else {
 #pragma unroll
@@ -236,19 +242,30 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8> struct Step {
 };
 
 // ------------------------------------------------------------------------------------------------ the walk
-template <typename T, int VE, int NS, int NT, bool AL8>
-__global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void paged_attn_k(const PagedP p) {
-    typedef Step<T, VE, NS, NT, AL8> S_t;
-    constexpr int SW = 16 * VE, DP = SW * NS, ST = 16 * NT, RD = 4 * ST, J = 4 * NT;      // a wave's step, a round of the four waves
-    constexpr int MERGE = 4 * 16 * SW * 4, QB = S_t::QFRAG;
-    __shared__ __attribute__((aligned(16))) char lds[QB > MERGE ? QB : MERGE];          // q fragments; at the end the waves' outputs
-    __shared__ __attribute__((aligned(16))) T own_k[DP], own_v[DP];
+// WPR: waves that share a (row, KV head, split): 4 (merged through LDS), or 1 (four of them side by side in a workgroup).  ST: the cache is
+// read past the last-level cache (non-temporal).
+template <typename T, int VE, int NS, int NT, bool AL8, int WPR, bool ST>
+__global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS * sizeof(T) * NT <= 48 ? 2 : 1)) void paged_attn_k(const PagedP p) {
+    typedef Step<T, VE, NS, NT, AL8, ST> S_t;
+    constexpr int SW = 16 * VE, DP = SW * NS, SL = 16 * NT, RD = WPR * SL, J = 4 * NT;    // a wave's step, a round of the waves of a row
+    constexpr int HEADS = WPR == 4 ? 16 : 4, QB = S_t::QT * HEADS * S_t::QS * (int)sizeof(T);   // query heads a tile may have (launch)
+    constexpr int MERGE = WPR == 4 ? 4 * 16 * SW * 4 : 0, TEAMS = 4 / WPR, TT = 64 * WPR;
+    __shared__ __attribute__((aligned(16))) char lds[TEAMS * QB > MERGE ? TEAMS * QB : MERGE];  // q; at the end the waves' outputs
+    __shared__ __attribute__((aligned(16))) T own_kv[TEAMS][2][DP];
     __shared__ float st_m[4][16], st_l[4][16];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), li = lane & 15, g = lane >> 4;
-    int id = blockIdx.x;
-    const int split = id % p.nsplit; id /= p.nsplit;
-    const int ct = id % p.ctiles; id /= p.ctiles;
-    const int hk = id % p.Hkv, b = id / p.Hkv;
+    const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
+    const int team = wv / WPR, wave = wv % WPR, tid = threadIdx.x % TT;                   // threads and waves of one team
+    T* qlds = (T*)(lds + team * QB);
+    T* own_k = own_kv[team][0]; T* own_v = own_kv[team][1];
+    auto sync = [&]() {                                                                   // the team's LDS is written
+        if constexpr (WPR == 4) lds_barrier();
+        else { __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront", "local"); __builtin_amdgcn_wave_barrier(); __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront", "local"); }
+    };
+    unsigned id = blockIdx.x * TEAMS + team;
+    if (WPR == 1 && id >= (unsigned)p.units) return;
+    const int split = (int)(id % (unsigned)p.nsplit); id /= (unsigned)p.nsplit;
+    const int ct = (int)(id % (unsigned)p.ctiles); id /= (unsigned)p.ctiles;
+    const int hk = (int)(id % (unsigned)p.Hkv), b = (int)(id / (unsigned)p.Hkv);
     const int d = p.d, cap = p.map.capacity(), len = p.lengths[b];
     const int h0 = hk * p.G + ct * 16, nh = min(16, p.G - ct * 16);                     // this tile's query heads
     const int n = min(max(len, 0), cap);                                                // slots in the cache
@@ -294,7 +311,7 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void page
         st.load_v(vp, vrow, d, li);
     };
     Pages e0, e1;
-    int s0 = lo + wave * ST;
+    int s0 = lo + wave * SL;
     const bool any = s0 < hi;                                                           // wave-uniform
     if (any) {
         fetch(s0, e0);
@@ -305,23 +322,24 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void page
     // ---- q (and the new key), rotated, while the first rows are under way
     const long trow = (long)paged_pos(p.positions, p.lengths, p.kn != nullptr, p.n_pos, b) * (p.rot >> 1);
     const float* cs = p.cos_t + trow; const float* sn = p.sin_t + trow;
-    if (nh < 16 || d < DP)
-        for (int i = tid; i < QB / 16; i += 256) *reinterpret_cast<u4_t*>(lds + i * 16) = u4_t{0u, 0u, 0u, 0u};
-    if (mine && d < DP) for (int c = d + tid; c < DP; c += 256) own_k[c] = own_v[c] = from_f<T>(0.f);
-    if (nh < 16 || d < DP) lds_barrier();
-    for (int i = tid; i < nh * d; i += 256) {
+    if (d < DP) {                                                                       // columns past d: zero, as in trim_k
+        const int pad = DP - d;
+        for (int i = tid; i < nh * pad; i += TT) S_t::put_q(qlds, HEADS, i / pad, d + i % pad, 0.f);
+        if (mine) for (int c = d + tid; c < DP; c += TT) own_k[c] = own_v[c] = from_f<T>(0.f);
+    }
+    for (int i = tid; i < nh * d; i += TT) {
         const int h = i / d, c = i - h * d;
-        S_t::put_q(lds, h, c, rotated((const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d, c, p.rot, cs, sn));
+        S_t::put_q(qlds, HEADS, h, c, rotated((const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d, c, p.rot, cs, sn));
     }
     if (mine)
-        for (int c = tid; c < d; c += 256) {
+        for (int c = tid; c < d; c += TT) {
             const T kv = from_f<T>(rotated((const T*)p.kn + (long)b * p.ld_k + (long)hk * d, c, p.rot, cs, sn));
             const T vv = ((const T*)p.vn)[(long)b * p.ld_v + (long)hk * d + c];
             own_k[c] = kv; own_v[c] = vv;
             if (own_row >= 0 && ct == 0) { ((T*)p.kpool)[own_row * d + c] = kv; ((T*)p.vpool)[own_row * d + c] = vv; }
         }
-    lds_barrier();
-    st.get_q(lds, lane);
+    sync();
+    const T* q = qlds + min(li, nh - 1) * S_t::QS + g * S_t::PE;                        // columns past the last head repeat it; nothing reads them
 
     f32x4_t acc[NS][VE];
 #pragma unroll
@@ -375,7 +393,7 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void page
     if (any) {
         for (; s0 + RD < hi; s0 += RD) {
             if (trim) st.trim_k(d, g);
-            st.scores(lds, lane, p.rot, s);
+            st.scores(q, HEADS, p.rot, s);
             load_k(s0 + RD, e1);
             weigh(s, ok, pr, s0);
             st.gather(pr, ok, vp, vrow, d, li, acc);
@@ -383,20 +401,40 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void page
             fetch(s0 + 2 * RD, e1);
         }
         if (trim) st.trim_k(d, g);
-        st.scores(lds, lane, p.rot, s);
+        st.scores(q, HEADS, p.rot, s);
         weigh(s, ok, pr, s0);
         st.gather(pr, ok, vp, vrow, d, li, acc);
     }
-    if (mine && own_row >= 0 && wave == (n - lo + ST - 1) / ST % 4) {                   // the new token: the wave whose turn it is
+    if (mine && own_row >= 0 && wave == (n - lo + SL - 1) / SL % WPR) {                   // the new token: the wave whose turn it is
         st.own_k(own_k, li, g);
-        st.scores(lds, lane, p.rot, s);
+        st.scores(q, HEADS, p.rot, s);
         weigh(s, lane < 16 ? 1u : 0u, pr, -1);
         st.gather_own(pr, own_v, li, g, acc);
     }
-    // ---- the four waves' parts; a wave without slots has m = -inf, l = 0 and weighs nothing
     l = quad_sum(l);
+    const bool single = p.nsplit == 1;
+    if constexpr (WPR == 1) {
+        const float inv = single ? (p.stable ? 1.f / fmaxf(l, 1e-9f) : l == 0.f ? 0.f : 1.f / l) : 1.f;
+        if (li >= nh) return;
+        const long bh = (long)b * p.H + h0 + li;
+        if (p.stat && g == 0) p.stat[bh * p.nsplit + split] = make_float2(p.stable ? 0.f : m, l);
+#pragma unroll
+        for (int a = 0; a < NS; a++)
+#pragma unroll
+            for (int r = 0; r < 4; r++)
+#pragma unroll
+                for (int e = 0; e < VE; e += 4) {
+                    const int c = a * SW + (g * 4 + r) * VE + e;
+                    const float x[4] = {acc[a][e][r] * inv, acc[a][e + 1][r] * inv, acc[a][e + 2][r] * inv, acc[a][e + 3][r] * inv};
+                    if (c >= d) continue;
+                    if (single) VecIO<T, 4>::store((T*)p.o + bh * d + c, x);
+                    else VecIO<float, 4>::store(p.part + (bh * p.nsplit + split) * d + c, x);
+                }
+        return;
+    }
+    // ---- the four waves' parts; a wave without slots has m = -inf, l = 0 and weighs nothing
     if (g == 0) { st_m[wave][li] = m; st_l[wave][li] = l; }
-    lds_barrier();                                                                      // also: the q fragments have been read
+    lds_barrier();                                                                      // also: q has been read
     float M = 0.f, L = 0.f, f = 1.f;
     if (!p.stable) {
         M = fmaxf(fmaxf(st_m[0][li], st_m[1][li]), fmaxf(st_m[2][li], st_m[3][li]));
@@ -408,7 +446,6 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) <= 24 ? 2 : 1)) void page
 #pragma unroll
         for (int w = 0; w < 4; w++) L += st_l[w][li];
     }
-    const bool single = p.nsplit == 1;
     if (p.stat && wave == 0 && g == 0 && li < nh) p.stat[((long)b * p.H + h0 + li) * p.nsplit + split] = make_float2(M, L);
     if (single) f *= p.stable ? 1.f / fmaxf(L, 1e-9f) : L == 0.f ? 0.f : 1.f / L;
     float* out = (float*)lds;
@@ -459,12 +496,12 @@ __device__ __forceinline__ void paged_final(const PagedP& p, long bh, int ns, fl
 }
 // Workgroups below `joins`: one (row, head): the splits' outputs, 256 / (d / 4) of them at a time, d / 4 lanes of 16 bytes each.
 // The others: 1024 slots of one (row, KV head): p = exp2(x - max) / sum (| s(x) / sum) of the group's heads, added to the slots' weights.
-template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const PagedP p, int joins, int wchunks) {
-    __shared__ __attribute__((aligned(16))) float red[256 * 4];
+template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join_k(const PagedP p, int joins, int wchunks) {
+    __shared__ __attribute__((aligned(16))) float red[NTH * 4];
     __shared__ float hb[64], hi[64];
     const int tid = threadIdx.x, wave = tid >> 6;
     if ((int)blockIdx.x < joins) {
-        const int bh = blockIdx.x, b = bh / p.H, cols = p.d >> 2, per = 256 / cols;
+        const int bh = blockIdx.x, b = bh / p.H, cols = p.d >> 2, per = NTH / cols;
         const int c = tid % cols, gr = tid / cols;
         const int ns = (paged_cover(p, b) + p.chunk - 1) / p.chunk;
         float base, inv;
@@ -487,7 +524,7 @@ template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const 
         return;
     }
     const int id = blockIdx.x - joins, ch = id % wchunks, bk = id / wchunks, b = bk / p.Hkv, hk = bk % p.Hkv;
-    const int n = paged_cover(p, b), s0 = ch * 1024;
+    const int n = paged_cover(p, b), s0 = ch * (NTH * 4);
     if (s0 >= n) return;
     const int ns = (n + p.chunk - 1) / p.chunk, cap = p.map.capacity();
     const int slot = s0 + tid * 4;
@@ -498,7 +535,7 @@ template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const 
         const int ng = min(64, p.G - g0);
         const long bh = (long)b * p.H + hk * p.G + g0;
         if (g0) __syncthreads();
-        for (int h = wave; h < ng; h += 4) {
+        for (int h = wave; h < ng; h += NTH / 64) {
             float base, inv;
             paged_final(p, bh + h, ns, base, inv);
             if ((tid & 63) == 0) { hb[h] = base; hi[h] = inv; }
@@ -523,14 +560,18 @@ template <typename T> __global__ __launch_bounds__(256) void paged_join_k(const 
     }
 }
 
-// How a cache of `cap` slots is split.  A workgroup takes whole rounds of 128 slots.
+// How a cache of `cap` slots is split, in whole rounds of 128: up to 512 slots not at all (a second launch costs more than it saves: 24.7 us
+// against 33.5 for 32 rows of 16 heads and 500 slots), else so that there are about 512 workgroups (1 row of 65551 slots, 4 KV heads: 38 us,
+// 44 with four times as many), and in parts of at most 1024 slots, which even out rows of different lengths (32 rows of 300 to 16384
+// slots, 8 KV heads: 249 us; 263 in parts of 512, whose outputs are twice as many).
 static int paged_chunk(int64_t tiles, int64_t cap) {
-    const int64_t want = 1024;
-    int64_t chunk = cdiv(cdiv(cap * tiles, want), 128) * 128;
+    int64_t chunk = cdiv(cap * tiles, 512);
     if (chunk > 1024) chunk = 1024;
     if (cap <= 512) chunk = cap;
     return (int)(cdiv(chunk, 128) * 128);
 }
+// Joining many splits takes a workgroup of 1024 threads (171 splits of 32 heads: 11 us with 256).
+static bool paged_wide_join(int nsplit) { return nsplit > 32; }
 struct PagedPlan { int chunk, nsplit; size_t part, stat, sc; };
 static PagedPlan paged_plan(const mm_paged_attn_args* a) {
     const int64_t cap = a->width * a->page, tiles = a->B * a->Hkv * cdiv(a->H / a->Hkv, 16);
@@ -550,8 +591,11 @@ extern "C" size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* a) {
     return r.part + r.stat + r.sc;
 }
 
-template <typename T, int VE, int NS, int NT, bool AL8> static void paged_launch(const PagedP& p, unsigned blocks, hipStream_t st) {
-    hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL8>), dim3(blocks), dim3(256), 0, st, p);
+template <typename T, int VE, int NS, int NT, bool AL8> static void paged_launch(const PagedP& p, bool lone, bool past, hipStream_t st) {
+#define MM_PAGED(WPR_, ST_) hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL8, WPR_, ST_>), dim3((unsigned)cdiv(p.units, WPR_ == 1 ? 4 : 1)), dim3(256), 0, st, p)
+    if (lone) { if (past) MM_PAGED(1, true); else MM_PAGED(1, false); }
+    else { if (past) MM_PAGED(4, true); else MM_PAGED(4, false); }
+#undef MM_PAGED
 }
 
 extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
@@ -580,34 +624,41 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     p.n_pos = a->rot ? (int)a->n_pos : 1; p.ld_q = a->ld_q; p.ld_k = a->ld_k; p.ld_v = a->ld_v; p.scale = (float)(1.0 / sqrt((double)a->d));
     p.chunk = r.chunk; p.nsplit = r.nsplit; p.ctiles = (int)cdiv(p.G, 16); p.stable = a->mode == MM_ATTN_STABLEMAX;
     const int64_t blocks = a->B * a->Hkv * p.ctiles * p.nsplit;
-    const int wchunks = a->weights ? (int)cdiv(a->width * a->page, 1024) : 0, joins = p.nsplit > 1 ? (int)(a->B * a->H) : 0;
+    const int wchunks = a->weights ? (int)cdiv(a->width * a->page, paged_wide_join(r.nsplit) ? 4096 : 1024) : 0, joins = p.nsplit > 1 ? (int)(a->B * a->H) : 0;
     const int64_t blocks2 = joins + a->B * a->Hkv * wchunks;
     MM_CHECK(a->B * a->H < (1LL << 31) && blocks < (1LL << 31) && blocks2 < (1LL << 31), "paged_decode_attn: too many rows and heads for one call");
-    const unsigned nb = (unsigned)blocks;
+    p.units = (int)blocks;
+    // Many short rows: a wave each (1024 rows of 160 to 238 slots, 8 heads: 164 us, four waves a row 173; 256 rows of 900, 8 KV heads: 150 and 140).
+    // A tile of more than four heads would not find its q in that variant's LDS.
+    const bool lone = p.G <= 4 && r.nsplit == 1 && a->width * a->page <= 512 && blocks >= 2048;
+    // A cache that the last-level cache (256 MB) cannot hold until the next call is read past it: 154 us for 164 at 849 MB; at 69 MB it
+    // would be 39 for 26.
+    const bool past = a->B * a->Hkv * a->width * a->page * a->d * (a->dtype == MM_BF16 ? 4 : 8) > (256LL << 20);
     const int64_t d = a->d;
     if (a->dtype == MM_F32) {
-        if (d <= 64) paged_launch<float, 4, 1, 2, true>(p, nb, st);
-        else if (d <= 128) paged_launch<float, 4, 2, 2, true>(p, nb, st);
-        else if (d <= 192) paged_launch<float, 4, 3, 2, true>(p, nb, st);
-        else if (d <= 256) paged_launch<float, 4, 4, 2, true>(p, nb, st);
-        else paged_launch<float, 4, 8, 1, true>(p, nb, st);
+        if (d <= 64) paged_launch<float, 4, 1, 1, true>(p, lone, past, st);
+        else if (d <= 128) paged_launch<float, 4, 2, 1, true>(p, lone, past, st);
+        else if (d <= 192) paged_launch<float, 4, 3, 1, true>(p, lone, past, st);
+        else if (d <= 256) paged_launch<float, 4, 4, 1, true>(p, lone, past, st);
+        else paged_launch<float, 4, 8, 1, true>(p, lone, past, st);
     } else if (d % 8 == 0) {
-        if (d <= 64) paged_launch<bf16, 4, 1, 2, true>(p, nb, st);
-        else if (d <= 128) paged_launch<bf16, 8, 1, 2, true>(p, nb, st);
-        else if (d <= 192) paged_launch<bf16, 4, 3, 2, true>(p, nb, st);
-        else if (d <= 256) paged_launch<bf16, 8, 2, 2, true>(p, nb, st);
-        else paged_launch<bf16, 8, 4, 2, true>(p, nb, st);
+        if (d <= 64) paged_launch<bf16, 4, 1, 2, true>(p, lone, past, st);
+        else if (d <= 128) paged_launch<bf16, 8, 1, 2, true>(p, lone, past, st);
+        else if (d <= 192) paged_launch<bf16, 4, 3, 2, true>(p, lone, past, st);
+        else if (d <= 256) paged_launch<bf16, 8, 2, 2, true>(p, lone, past, st);
+        else paged_launch<bf16, 8, 4, 1, true>(p, lone, past, st);
     } else {                                                                            // rows of whole 8-byte pieces only
-        if (d <= 64) paged_launch<bf16, 4, 1, 2, false>(p, nb, st);
-        else if (d <= 128) paged_launch<bf16, 4, 2, 2, false>(p, nb, st);
-        else if (d <= 192) paged_launch<bf16, 4, 3, 2, false>(p, nb, st);
-        else if (d <= 256) paged_launch<bf16, 4, 4, 2, false>(p, nb, st);
-        else paged_launch<bf16, 4, 8, 2, false>(p, nb, st);
+        if (d <= 64) paged_launch<bf16, 4, 1, 2, false>(p, lone, past, st);
+        else if (d <= 128) paged_launch<bf16, 4, 2, 2, false>(p, lone, past, st);
+        else if (d <= 192) paged_launch<bf16, 4, 3, 2, false>(p, lone, past, st);
+        else if (d <= 256) paged_launch<bf16, 4, 4, 2, false>(p, lone, past, st);
+        else paged_launch<bf16, 4, 8, 1, false>(p, lone, past, st);
     }
     MM_LAUNCH_CHECK();
     if (blocks2) {
-        if (a->dtype == MM_F32) hipLaunchKernelGGL(paged_join_k<float>, dim3((unsigned)blocks2), dim3(256), 0, st, p, joins, wchunks);
-        else hipLaunchKernelGGL(paged_join_k<bf16>, dim3((unsigned)blocks2), dim3(256), 0, st, p, joins, wchunks);
+#define MM_JOIN(T_) do { if (paged_wide_join(r.nsplit)) hipLaunchKernelGGL((paged_join_k<T_, 1024>), dim3((unsigned)blocks2), dim3(1024), 0, st, p, joins, wchunks); \
+                         else hipLaunchKernelGGL((paged_join_k<T_, 256>), dim3((unsigned)blocks2), dim3(256), 0, st, p, joins, wchunks); } while (0)
+        if (a->dtype == MM_F32) MM_JOIN(float); else MM_JOIN(bf16);
         MM_LAUNCH_CHECK();
     }
     return MM_OK;
