@@ -19,9 +19,11 @@ __device__ __forceinline__ unsigned weight_key(float x) {
 }
 struct EvictP {
     char* kpool; char* vpool; float* w; int* lengths; int* kept; PagedMap map;
-    int* ws;                       // per (row, KV head): {slots, moves}, then targets [room] and sources [room] of the moves
-    int room, units, budget, recent, B;                                        // units: 16- or 8-byte pieces of a slot's K
-    __device__ __forceinline__ int* head(long bh) const { return ws + bh * (2L * room + 4); }
+    char* ws; int room;            // per (row, KV head): {slots, moves}; pool rows to [room] and from [room] of the moves; the same as slots
+    int units, budget, recent;                                                 // units: 16- or 8-byte pieces of a slot's K
+    __device__ __forceinline__ int* head(long bh) const { return (int*)(ws + bh * (24L * room + 16)); }
+    __device__ __forceinline__ long* rows(long bh) const { return (long*)(head(bh) + 4); }
+    __device__ __forceinline__ int* slots(long bh) const { return (int*)(rows(bh) + 2L * room); }
 };
 
 // ------------------------------------------------------------------------------------------------ selection (NW waves)
@@ -51,7 +53,7 @@ template <int NW> __device__ __forceinline__ int block_scan(int v, int* red, int
 }
 
 // R registers of keys a thread (four consecutive slots a round), R = 0: read again in every pass
-template <int NW, int R> __device__ void evict_select(const EvictP& p, int b, int h, int* red) {
+template <int NW, int R> __device__ __forceinline__ void evict_select(const EvictP& p, int b, int h, int* red) {
     constexpr int ROUND = NW * 256;
     const long bh = (long)b * p.map.Hkv + h;
     const int tid = threadIdx.x, n = min(p.lengths[b], p.map.capacity());
@@ -63,7 +65,10 @@ template <int NW, int R> __device__ void evict_select(const EvictP& p, int b, in
         return;
     }
     const int A = p.budget - p.recent, old = n - p.recent, rounds = (old + ROUND - 1) / ROUND;
-    int* to = hd + 4; int* from = to + p.room;
+    // the moves as slots: in LDS where they fit (at most half of the slots move)
+    constexpr int LIST = R > 0 && NW * R * 64 <= 8192 ? NW * R * 32 : 0;
+    __shared__ int list[LIST ? 2 * LIST : 1];
+    int* to = LIST ? list : p.slots(bh); int* from = to + (LIST ? LIST : p.room);
     auto load = [&](int r, unsigned (&k)[4]) {
         const int s = r * ROUND + tid * 4;                                     // four slots of one page
         const long row = s < old ? p.map.row(b, h, s) : -1;
@@ -146,15 +151,34 @@ template <int NW, int R> __device__ void evict_select(const EvictP& p, int b, in
     __syncthreads();                                                           // the lists are written
     const int moves = min(holes, late);
     if (tid == 0) hd[1] = moves;
-    for (int i = tid; i < moves; i += NW * 64) kept[to[i]] = from[i];
+    long* rows = p.rows(bh);                                                   // looked up once here, not once a piece
+    constexpr int N = 4;
+    for (int i0 = tid; i0 < moves; i0 += NW * 64 * N) {
+        int ts[N], fs[N];
+        long rt[N], rf[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) {
+            const int i = i0 + j * NW * 64;
+            ts[j] = i < moves ? to[i] : -1; fs[j] = i < moves ? from[i] : -1;
+        }
+#pragma unroll
+        for (int j = 0; j < N; j++) { rt[j] = p.map.row(b, h, ts[j]); rf[j] = p.map.row(b, h, fs[j]); }
+#pragma unroll
+        for (int j = 0; j < N; j++)
+            if (ts[j] >= 0) {
+                const int i = i0 + j * NW * 64;
+                kept[ts[j]] = fs[j];
+                rows[i] = rf[j] < 0 ? -1 : rt[j]; rows[p.room + i] = rf[j];
+            }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ moving
 // independent moves [first, ..) of a (row, KV head), one piece of K and of V a thread; `step` threads share the work
 template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& p, int b, int h, int t, int step) {
-    const int* hd = p.head((long)b * p.map.Hkv + h);
-    const int* to = hd + 4; const int* from = to + p.room;
-    const unsigned total = (unsigned)hd[1] * (unsigned)p.units;
+    const long bh = (long)b * p.map.Hkv + h;
+    const long* to = p.rows(bh); const long* from = to + p.room;
+    const unsigned total = (unsigned)p.head(bh)[1] * (unsigned)p.units;
     U* K = (U*)p.kpool; U* V = (U*)p.vpool;
     constexpr int N = 4;                                                       // in flight
     for (unsigned i0 = t; i0 < total; i0 += (unsigned)step * N) {
@@ -169,9 +193,9 @@ template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& 
             if (i < total) {
                 const unsigned m = i / (unsigned)p.units;
                 piece[j] = (int)(i - m * (unsigned)p.units);
-                const long s = p.map.row(b, h, from[m]);
-                if (s >= 0) {
-                    d[j] = p.map.row(b, h, to[m]);
+                const long s = from[m];
+                d[j] = to[m];
+                if (d[j] >= 0) {
                     k[j] = K[s * p.units + piece[j]]; v[j] = V[s * p.units + piece[j]];
                     if (piece[j] == 0) w[j] = p.w[s];
                 }
@@ -236,16 +260,19 @@ template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW *
         evict_shift<U>(p, b, h, threadIdx.x, NW * 64);
     }
 }
-template <typename U> __global__ __launch_bounds__(256) void evict_moves_k(const EvictP p) {
+// The last launch writes the new lengths: only the selection reads the old ones.
+__device__ __forceinline__ void evict_length(const EvictP& p, int b) {
+    if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.head((long)b * p.map.Hkv)[0] > p.budget) p.lengths[b] = p.budget;
+}
+template <typename U, bool LAST> __global__ __launch_bounds__(256) void evict_moves_k(const EvictP p) {
     evict_moves<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
+    if constexpr (LAST) evict_length(p, blockIdx.x);
 }
 template <typename U> __global__ __launch_bounds__(256) void evict_shift_k(const EvictP p) {
     evict_shift<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
+    evict_length(p, blockIdx.x);
 }
-__global__ void evict_lengths_k(const EvictP p) {                              // in a launch of its own: every head's workgroup reads the old ones
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b < p.B && p.lengths[b] > p.budget && p.map.capacity() > p.budget) p.lengths[b] = p.budget;
-}
+__global__ __launch_bounds__(64) void evict_lengths_k(const EvictP p) { evict_length(p, blockIdx.x); }
 
 static int64_t evict_room(int64_t page, int64_t width, int64_t budget, int64_t recent) {
     const int64_t cap = page * width, A = budget - recent;
@@ -253,29 +280,34 @@ static int64_t evict_room(int64_t page, int64_t width, int64_t budget, int64_t r
 }
 extern "C" size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page, int64_t width, int64_t budget, int64_t recent) {
     if (B <= 0 || Hkv <= 0 || page <= 0 || width <= 0 || recent < 0 || budget < recent) return 0;
-    return (size_t)(B * Hkv) * (size_t)(2 * evict_room(page, width, budget, recent) + 4) * sizeof(int);
+    return (size_t)(B * Hkv) * (size_t)(24 * evict_room(page, width, budget, recent) + 16);
 }
 
-template <typename U> static void evict_launch(const EvictP& p, int64_t cap, int64_t max_moves, hipStream_t st) {
-    const dim3 grid((unsigned)p.B, (unsigned)p.map.Hkv);
-    const int64_t heads = (int64_t)p.B * p.map.Hkv;
-    // one launch does everything where there are rows and heads enough to fill the card, or little to move
-    const bool all = heads >= 128 || (max_moves + p.recent) * p.units <= 8192;
+template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64_t cap, hipStream_t st) {
+    const dim3 grid((unsigned)B, (unsigned)p.map.Hkv);
+    const int64_t heads = B * p.map.Hkv;
+    // One workgroup does everything where there is little to move; else the moves and the shift spread over the card in launches of their
+    // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 181 in three).
+    const bool all = ((int64_t)p.room + p.recent) * p.units <= 8192;
 #define MM_SELECT(NW_, R_) do { if (all) hipLaunchKernelGGL((evict_select_k<NW_, R_, U, true>), grid, dim3(NW_ * 64), 0, st, p); \
                                 else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
-    if (cap <= 1024) MM_SELECT(4, 4);
-    else if (cap <= 8192) MM_SELECT(16, 8);
-    else if (cap <= 32768) MM_SELECT(16, 32);
-    else if (cap <= 65536) MM_SELECT(16, 64);
+    if (cap <= 1024) MM_SELECT(4, 4);                                          // eight waves: fewer share a barrier's price (8192 slots: 26 us, 16 waves 37, 4 waves 33)
+    else if (cap <= 8192) MM_SELECT(8, 16);
+    else if (cap <= 32768) MM_SELECT(8, 64);
+    else if (cap <= 65536) MM_SELECT(8, 128);
     else MM_SELECT(16, 0);
 #undef MM_SELECT
-    if (all) return;
     auto split = [&](int64_t items) {                                          // workgroups per (row, KV head): four pieces a thread, 4096 workgroups in all
         const int64_t w = cdiv(items, 1024), most = cdiv(4096, heads);
         return (unsigned)(w < 1 ? 1 : w < most ? w : most);
     };
-    if (max_moves) hipLaunchKernelGGL(evict_moves_k<U>, dim3(grid.x, grid.y, split(max_moves * p.units)), dim3(256), 0, st, p);
-    if (p.recent) hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, split((int64_t)p.recent * p.units)), dim3(256), 0, st, p);
+    if (!all && p.room) {
+        const dim3 g(grid.x, grid.y, split((int64_t)p.room * p.units));
+        if (p.recent) hipLaunchKernelGGL((evict_moves_k<U, false>), g, dim3(256), 0, st, p);
+        else hipLaunchKernelGGL((evict_moves_k<U, true>), g, dim3(256), 0, st, p);
+    }
+    if (!all && p.recent) hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, split((int64_t)p.recent * p.units)), dim3(256), 0, st, p);
+    if (all) hipLaunchKernelGGL(evict_lengths_k, dim3(grid.x), dim3(64), 0, st, p);
 }
 
 extern "C" int mm_paged_evict(void* kpool, void* vpool, float* weights, const int32_t* page_table, int32_t* lengths, int32_t* kept, int64_t B,
@@ -288,19 +320,18 @@ extern "C" int mm_paged_evict(void* kpool, void* vpool, float* weights, const in
     if (B == 0) return MM_OK;
     MM_CHECK(weights && lengths && kept && workspace, "paged_evict: null pointer");
     MM_CHECK(((uintptr_t)weights % 16) == 0, "paged_evict: weights must be 16-byte aligned");
-    MM_CHECK(workspace_bytes >= mm_paged_evict_workspace(B, Hkv, page, width, budget, recent), "paged_evict: workspace too small");
+    MM_CHECK(workspace_bytes >= mm_paged_evict_workspace(B, Hkv, page, width, budget, recent) && ((uintptr_t)workspace % 16) == 0,
+             "paged_evict: workspace too small or not 16-byte aligned");
     const int64_t bytes = d * (dtype == MM_BF16 ? 2 : 4), room = evict_room(page, width, budget, recent);
     const int piece = bytes % 16 == 0 ? 16 : 8;
     MM_CHECK((room + recent) * (bytes / piece) < (1LL << 31), "paged_evict: too many slots for one call");
     EvictP p{};
     p.kpool = (char*)kpool; p.vpool = (char*)vpool; p.w = weights; p.lengths = lengths; p.kept = kept;
     p.map = {page_table, (long)ld_table, (int)width, paged_shift(page), (int)n_pages, (int)Hkv};
-    p.ws = (int*)workspace; p.room = (int)room; p.units = (int)(bytes / piece); p.budget = (int)budget; p.recent = (int)recent; p.B = (int)B;
+    p.ws = (char*)workspace; p.room = (int)room; p.units = (int)(bytes / piece); p.budget = (int)budget; p.recent = (int)recent;
     hipStream_t st = (hipStream_t)stream;
-    if (piece == 16) evict_launch<mm_u4_t>(p, page * width, room, st);
-    else evict_launch<mm_u2_t>(p, page * width, room, st);
-    MM_LAUNCH_CHECK();
-    hipLaunchKernelGGL(evict_lengths_k, dim3((unsigned)cdiv(B, 256)), dim3(256), 0, st, p);
+    if (piece == 16) evict_launch<mm_u4_t>(p, B, page * width, st);
+    else evict_launch<mm_u2_t>(p, B, page * width, st);
     MM_LAUNCH_CHECK();
     return MM_OK;
 }
