@@ -25,6 +25,34 @@ class KVCache:
         self.Smax = Smax
 
 
+class PagedKVCache:
+    """Keys and values of every layer in pages of `page` slots (ops.paged_decode_attn): rows may hold any number of slots, up to `slots`.
+    One page table serves all layers; lengths[b] is what row b holds.  weights=True keeps the attention each slot has drawn, by which
+    evict() cuts rows down."""
+
+    def __init__(self, n_layers: int, B: int, H: int, slots: int, d: int, page: int, dtype, device, weights: bool = False):
+        width = -(-slots // page)
+        pool = lambda: torch.empty((B * width, H, page, d), dtype=dtype, device=device)
+        self.k, self.v = [pool() for _ in range(n_layers)], [pool() for _ in range(n_layers)]
+        self.w = [torch.empty((B * width, H, page), dtype=torch.float32, device=device) if weights else None for _ in range(n_layers)]
+        self.page_table = torch.arange(B * width, dtype=torch.int32, device=device).view(B, width)
+        self.lengths = torch.zeros(B, dtype=torch.int32, device=device)
+
+    def fill(self, li: int, k, v, rot: int, cos_t, sin_t, start=None):
+        ops.paged_cache_fill(k, v, self.k[li], self.v[li], self.page_table, rot, cos_t, sin_t, start=start, weights=self.w[li])
+
+    def attend(self, li: int, q, k_new, v_new, H: int, rot: int, cos_t, sin_t, stablemax: bool, positions=None):
+        return ops.paged_decode_attn(q, k_new, v_new, self.k[li], self.v[li], self.page_table, self.lengths, H, rot, cos_t, sin_t, stablemax,
+                                     positions=positions, weights=self.w[li])
+
+    def evict(self, budget: int, recent: int):
+        """Every row and layer down to `budget` slots: the `recent` newest and the most attended (ops.paged_evict)."""
+        for k, v, w in zip(self.k, self.v, self.w):
+            n = self.lengths.clone()
+            ops.paged_evict(k, v, w, self.page_table, n, budget, recent)
+        self.lengths = n
+
+
 def _layer_weights(layer, dt):
     """GEMM operands of one layer from the operand cache (functional.cached_operand: built once per parameter version,
     refreshed by the optimizer -- nothing is re-cast or re-concatenated per generate() call).  Weights in the compute
@@ -67,6 +95,56 @@ def _lin(x2, w, b, b16=None, act=0, res=None, out_dtype=None, square=False):
     if res is not None:
         y.add_(res)
     return y if out_dtype in (None, y.dtype) else y.to(out_dtype)
+
+
+def _rows_logits(dec, weights, h, attend, w_out, b_out, b_out16):
+    """Decoder layers over rows of single tokens, h [rows, E] -> float32 logits [rows, V]; attend(layer number, layer, qkv [rows, 3E]) -> [rows, E]."""
+    for li, layer in enumerate(dec.layers):
+        w = weights[li]
+        # LN, QKV (+bias), K4, out-proj (+bias +residual fused), LN, W1 (+bias) relu^2, W2 (+bias) += residual; operands
+        # and bias copies come from the operand cache (no per-call casts)
+        xa, _, _ = ops.layernorm_fwd(h, layer.attn_norm.weight, layer.attn_norm.bias)
+        qkv = _lin(xa, w["wqkv"], w["bqkv"], w["bqkv16"])                      # [rows, 3E]
+        h = _lin(attend(li, layer, qkv), w["wo"], w["bo"], res=h, square=True)
+        xf, _, _ = ops.layernorm_fwd(h, layer.mlp_norm.weight, layer.mlp_norm.bias)
+        u = _lin(xf, w["w1"], w["b1"], w["b116"], act=ops.ACT_RELU2, square=True)      # libmmhip: bias + relu^2 fused
+        h = _lin(u, w["w2"], w["b2"], w["b216"], res=h)
+    xt, _, _ = ops.layernorm_fwd(h, dec.final_norm.weight, dec.final_norm.bias)
+    return _lin(xt, w_out, b_out, b_out16, out_dtype=torch.float32)
+
+
+def _prefill(dec, weights, prompt, Smax, store):
+    """Pass over the PROMPT rows [b, P, E] (prompt positions see each other and nothing else, so they do not depend on what follows);
+    store(layer number, k, v, rot, cos, sin) takes every layer's keys and values.  The BOS token is not part of it -- it is decode step 0
+    at position P -- and of the last layer only the keys and values of the prompt are computed: nothing reads that layer's outputs
+    at prompt positions (its attention, out-projection and MLP over B*P rows were a fifth of the prefill's products)."""
+    x = prompt.contiguous()
+    nb, S0, E = x.shape
+    H, M0, dt = dec.num_heads, nb * S0, x.dtype
+    for li, layer in enumerate(dec.layers):
+        w = weights[li]
+        cos_t, sin_t = layer.rotary_emb.half_tables(Smax)
+        xa, _, _ = ops.layernorm_fwd(x, layer.attn_norm.weight, layer.attn_norm.bias)
+        rot = layer.rotary_ndims
+        if li == len(dec.layers) - 1:
+            kv = torch.addmm(w["bqkv16"][E:], xa.view(M0, E), w["wqkv"][E:].t()).view(nb, S0, 2, E)
+            if dt == torch.bfloat16 and rot > 0:
+                ops.rope_inplace(kv.view(nb, S0, 2 * E)[:, :, :E], H, rot, cos_t, sin_t)
+                rot = 0
+            store(li, kv[:, :, 0], kv[:, :, 1], rot, cos_t, sin_t)
+            break
+        # the big prefill products stay on the library where it wins (N = 3E, 4E), the N = E products with
+        # their bias + residual run on the large-tile kernel, as in the training forward
+        qkv = torch.addmm(w["bqkv16"], xa.view(M0, E), w["wqkv"].t()).view(nb, S0, 3, E)
+        if dt == torch.bfloat16 and rot > 0:   # rotate q,k once in place: cache fill becomes a copy, K3 runs its fast form
+            ops.rope_inplace(qkv.view(nb, S0, 3 * E)[:, :, :2 * E], 2 * H, rot, cos_t, sin_t)
+            rot = 0
+        store(li, qkv[:, :, 1], qkv[:, :, 2], rot, cos_t, sin_t)
+        a, _ = ops.prefix_attn_fwd(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], H, rot, S0, cos_t, sin_t, layer.use_stablemax)
+        x = _lin(a.view(M0, E), w["wo"], w["bo"], res=x.view(M0, E), square=True).view(nb, S0, E)
+        xf, _, _ = ops.layernorm_fwd(x, layer.mlp_norm.weight, layer.mlp_norm.bias)
+        u = ops.relu2_fwd(torch.addmm(w["b116"], xf.view(M0, E), w["w1"].t()))     # fused on libmmhip it measured slower (prefill 27.5 vs 25 ms)
+        x = _lin(u, w["w2"], w["b2"], res=x.view(M0, E), square=True).view(nb, S0, E)  # prefill: N = E on the large-tile kernel
 
 
 class _StepPlan:
@@ -180,11 +258,157 @@ class _StepPlan:
                     L.check(rc, name)
 
 
+class _PagedDecoder:
+    """A model's decoder over a paged cache: prompts of one batch stored, then tokens row by row.  cache.lengths[b] is what row b holds (the
+    caller advances it; < 0: the row sits out), positions its next rotary position where that is not the same."""
+
+    def __init__(self, model, nmr_tokens, ir_data, slots, positions: int, page: int, weights: bool = False):
+        """slots: function of the prompt's length -> slots per row; positions: tokens behind the prompt that the rotary tables have to hold."""
+        dec = self.dec = model.decoder
+        dt = self.dt = FN.get_compute_dtype()
+        prompt = dec.build_prompt(model.encoder(None, ir_data, None), nmr_tokens, dt)
+        B, self.P, E = prompt.shape
+        self.H, self.E, self.Smax = dec.num_heads, E, self.P + positions
+        self.weights = [_layer_weights(l, dt) for l in dec.layers]
+        self.out = (FN.cached_operand((dec.out.weight,), dt), dec.out.bias.detach(), FN.cached_operand((dec.out.bias,), dt))
+        self.cache = PagedKVCache(len(dec.layers), B, self.H, slots(self.P), E // self.H, page, dt, prompt.device, weights)
+        _prefill(dec, self.weights, prompt, self.Smax, self.cache.fill)
+        self.cache.lengths.fill_(self.P)
+
+    def step(self, ids: torch.Tensor, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token of every row, ids [B] -> logits [B, V]."""
+        E = self.E
+
+        def attend(li, layer, qkv):
+            return self.cache.attend(li, qkv[:, :E], qkv[:, E:2 * E], qkv[:, 2 * E:], self.H, layer.rotary_ndims,
+                                     *layer.rotary_emb.half_tables(self.Smax), layer.use_stablemax, positions=positions)
+        return _rows_logits(self.dec, self.weights, self.dec.smiles_embed.weight[ids].to(self.dt), attend, *self.out)
+
+    def run(self, ids: torch.Tensor) -> torch.Tensor:
+        """T tokens of every row at once, ids [B, T] -> logits [B, T, V]: each layer stores the run's keys and values, then every token
+        attends as a row of its own, over the slots up to its own."""
+        B, T = ids.shape
+        E, c = self.E, self.cache
+        n = c.lengths
+        upto = n[:, None] + torch.arange(1, T + 1, dtype=torch.int32, device=n.device)
+        upto = torch.where(n[:, None] < 0, torch.full_like(upto, -1), upto).reshape(-1)
+        table = c.page_table.repeat_interleave(T, 0)
+
+        def attend(li, layer, qkv):
+            cos_t, sin_t = layer.rotary_emb.half_tables(self.Smax)
+            run = qkv.view(B, T, 3 * E)
+            c.fill(li, run[:, :, E:2 * E], run[:, :, 2 * E:], layer.rotary_ndims, cos_t, sin_t, start=n)
+            return ops.paged_decode_attn(qkv[:, :E], None, None, c.k[li], c.v[li], table, upto, self.H, layer.rotary_ndims, cos_t, sin_t,
+                                         layer.use_stablemax)
+        h = self.dec.smiles_embed.weight[ids.reshape(-1)].to(self.dt)
+        return _rows_logits(self.dec, self.weights, h, attend, *self.out).view(B, T, -1)
+
+
+def _paged_greedy(model, nmr_tokens, ir_data, max_len, bos_id, eos_id, early_stop, sync_every, page_size, kv_budget, kv_recent):
+    dec = model.decoder
+    steps = min(max_len, dec.max_seq_length)
+    grow = max(1, kv_recent)                           # tokens between two evictions
+    slots = lambda P: P + steps if kv_budget is None else min(P + steps, max(kv_budget, P) + grow)
+    pd = _PagedDecoder(model, nmr_tokens, ir_data, slots, steps, page_size, weights=kv_budget is not None)
+    P, c = pd.P, pd.cache
+    if P + steps > dec.max_seq_length + 256:
+        steps = dec.max_seq_length + 256 - P           # the reference's length guard, as in the dense cache's loop
+    B, dev = c.lengths.shape[0], c.lengths.device
+    tokens = torch.full((B, steps + 1), bos_id, dtype=torch.long, device=dev)
+    finished = torch.zeros(B, dtype=torch.bool, device=dev)
+    positions = c.lengths.clone()
+    held, limit, n_done = P, None if kv_budget is None else max(kv_budget, P) + grow, 0
+    for t in range(steps):
+        if early_stop and t > 0 and t % sync_every == 0 and bool(finished.all()):
+            break
+        tokens[:, t + 1] = ops.argmax_rows(pd.step(tokens[:, t], positions))
+        finished.logical_or_(tokens[:, t + 1] == eos_id)
+        c.lengths.add_(1); positions.add_(1)
+        held, n_done = held + 1, t + 1
+        if limit is not None and held >= limit:
+            c.evict(kv_budget, kv_recent)
+            held, limit = kv_budget, kv_budget + grow
+    return tokens[:, : n_done + 1]
+
+
+@torch.no_grad()
+def speculative_generate(model, draft, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Tensor, max_len: int = 128, bos_id: int = 12,
+                         eos_id: int = 13, pad_id: int = 0, n_draft: int = 4, temperature: float = 1.0,
+                         generator: Optional[torch.Generator] = None, page_size: int = 16) -> torch.Tensor:
+    """Sampled decoding of `model` with tokens drafted by `draft`, a smaller model over the same vocabulary: the draft proposes n_draft tokens
+    one by one, the model looks at all of them in one pass, and ops.verify_drafts accepts the longest run that leaves the tokens
+    distributed as the model's own samples at this temperature.  Rows accept different numbers of tokens, so their caches are paged.
+    temperature=0: greedy, the ids of generate() up to each row's end (near-ties aside: the passes are of other shapes).  Returns int64
+    [B, <= max_len+1]: BOS, the tokens up to EOS or max_len of them, then pad_id."""
+    if n_draft < 1 or temperature < 0:
+        raise ValueError(f"speculative_generate: n_draft={n_draft} (at least 1), temperature={temperature} (not negative)")
+    if model.decoder.out.weight.shape[0] != draft.decoder.out.weight.shape[0]:
+        raise ValueError("speculative_generate: model and draft must share one vocabulary")
+    FN.flush_deferred_updates()
+    was_training = model.training, draft.training
+    model.eval(); draft.eval()
+    try:
+        T = n_draft + 1
+        steps = min(max_len, model.decoder.max_seq_length, draft.decoder.max_seq_length)
+        sides = [_PagedDecoder(m, nmr_tokens, ir_data, lambda P: P + steps + T, steps + T, page_size) for m in (model, draft)]
+        for m, s in zip((model, draft), sides):
+            steps = min(steps, m.decoder.max_seq_length + 256 - s.P)
+        target, helper = sides
+        B, dev = target.cache.lengths.shape[0], target.cache.lengths.device
+        rand = lambda n: torch.rand(B, n, generator=generator, device=dev)
+        none = torch.empty((B, 0), dtype=torch.long, device=dev)
+        col = torch.arange(T, device=dev)
+        out = torch.full((B, steps + 1 + T), pad_id, dtype=torch.long, device=dev)
+        out[:, 0] = bos_id
+        cur, said = out[:, 0].clone(), torch.zeros(B, dtype=torch.long, device=dev)
+        done = torch.zeros(B, dtype=torch.bool, device=dev)
+        held = [s.cache.lengths.clone() for s in sides]
+
+        def probabilities(logits):
+            if temperature == 0:
+                best = ops.argmax_rows(logits.reshape(-1, logits.shape[-1])).view(logits.shape[:-1])
+                return torch.zeros_like(logits).scatter_(-1, best[..., None], 1.0)
+            return torch.softmax(logits / temperature, -1)
+        while steps > 0:
+            for s, n in zip(sides, held):
+                s.cache.lengths = torch.where(done, torch.full_like(n, -1), n)
+            ids, q = [cur], []
+            for i in range(T):                         # the last step only stores the last draft's key and value
+                p = helper.step(ids[-1])
+                helper.cache.lengths = torch.where(done, helper.cache.lengths, helper.cache.lengths + 1)
+                if i < n_draft:
+                    q.append(probabilities(p))
+                    ids.append(ops.verify_drafts(none, q[-1][:, None], rand(1))[0][:, 0])
+            ids = torch.stack(ids, 1)
+            p = probabilities(target.run(ids))
+            new, accepted = ops.verify_drafts(ids[:, 1:], p, rand(T), q=None if temperature == 0 else torch.stack(q, 1))
+            accepted = accepted.long()
+            end = torch.where((new == eos_id) & (col <= accepted[:, None]), col, T).amin(1)          # T: no EOS among them
+            keep = col <= torch.minimum(accepted, end)[:, None]
+            at = said[:, None] + 1 + col
+            out.scatter_(1, at, torch.where(done[:, None], out.gather(1, at), torch.where(keep, new, torch.full_like(new, pad_id))))
+            cur = new.gather(1, accepted[:, None])[:, 0]
+            more = torch.where(done, torch.zeros_like(accepted), accepted + 1)
+            said += more
+            held = [n + more.to(torch.int32) for n in held]
+            done = done | (end < T) | (said >= steps)
+            if bool(done.all()):
+                break
+        return out[:, : min(steps, int(said.max())) + 1] if steps > 0 else out[:, :1]
+    finally:
+        model.train(was_training[0]); draft.train(was_training[1])
+
+
 @torch.no_grad()
 def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Tensor, max_len: int = 128, bos_id: int = 12,
-                    eos_id: int = 13, early_stop: bool = True, sync_every: int = 8,
-                    graph: Optional[bool] = None) -> torch.Tensor:
-    """graph=True: replay the decode step from ONE captured HIP graph (position, output column and current ids live in device
+                    eos_id: int = 13, early_stop: bool = True, sync_every: int = 8, graph: Optional[bool] = None,
+                    page_size: Optional[int] = None, kv_budget: Optional[int] = None, kv_recent: int = 16) -> torch.Tensor:
+    """page_size: keep the keys and values in pages of so many slots (PagedKVCache) instead of one dense array per layer.  kv_budget: keep at
+    most so many slots of a row between evictions (page_size defaults to 16): every kv_recent tokens each layer's heads drop the older
+    slots that have drawn the least attention, and the kv_recent newest always stay; memory per row is then bounded, and the ids are
+    those of the pruned attention.
+
+    graph=True: replay the decode step from ONE captured HIP graph (position, output column and current ids live in device
     memory and advance inside the graph).  Same kernels, same ids as the eager loop (tested), but OFF by default: on this
     stack (ROCm 7.2) replaying the ~45-node step costs more than issuing it -- nocat shape, 80 steps: B=1024 549k vs 643k
     tokens/s eager, B=128 181k vs 178k -- the decode loop is not host-bound (unlike the small-config train step, where
@@ -194,6 +418,15 @@ def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Te
     FN.flush_deferred_updates()        # this loop reads the weights directly, not through model.forward (optim: deferred updates)
     was_training = model.training
     model.eval()
+    if page_size is not None or kv_budget is not None:
+        if graph:
+            raise ValueError("greedy_generate: graph=True runs on the dense cache only")
+        if kv_budget is not None and not 0 < kv_recent <= kv_budget:
+            raise ValueError(f"greedy_generate: kv_recent={kv_recent} must be between 1 and kv_budget={kv_budget}")
+        try:
+            return _paged_greedy(model, nmr_tokens, ir_data, max_len, bos_id, eos_id, early_stop, sync_every, page_size or 16, kv_budget, kv_recent)
+        finally:
+            model.train(was_training)
     dev = ir_data.device
     B = nmr_tokens.size(0) if nmr_tokens is not None else ir_data.size(0)
     steps = min(max_len, dec.max_seq_length)                                   # train_autoregressive.py:91
@@ -216,67 +449,21 @@ def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Te
     for layer in dec.layers:
         layer.rotary_emb.half_tables(Smax)         # cached tables exist before any other stream asks for them
 
-    def prefill(pr, kcs, vcs):
-        """Pass over the PROMPT rows `pr` [b, P, E] on the current stream (prompt positions see each other and nothing else, so
-        they do not depend on what follows): fills the rows' cache slices (kcs / vcs: per-layer [b, H, Smax, d]).  The BOS
-        token is not part of it -- it is decode step 0 at position P -- and of the last layer only the keys and values of the
-        prompt are computed: nothing reads that layer's outputs at prompt positions (its attention, out-projection and MLP over
-        B*P rows were a fifth of the prefill's products)."""
-        nb = pr.shape[0]
-        x = pr.contiguous()
-        S0 = P
-        M0 = nb * S0
-        for li, layer in enumerate(dec.layers):
-            w = weights[li]
-            cos_t, sin_t = layer.rotary_emb.half_tables(Smax)
-            xa, _, _ = ops.layernorm_fwd(x, layer.attn_norm.weight, layer.attn_norm.bias)
-            rot = layer.rotary_ndims
-            if li == len(dec.layers) - 1:
-                kv = torch.addmm(w["bqkv16"][E:], xa.view(M0, E), w["wqkv"][E:].t()).view(nb, S0, 2, E)
-                if dt == torch.bfloat16 and rot > 0:
-                    ops.rope_inplace(kv.view(nb, S0, 2 * E)[:, :, :E], H, rot, cos_t, sin_t)
-                    rot = 0
-                ops.kv_cache_fill(kv[:, :, 0], kv[:, :, 1], kcs[li], vcs[li], H, rot, cos_t, sin_t)
-                break
-            # the big prefill products stay on the library where it wins (N = 3E, 4E: DESIGN.md 4), the N = E products with
-            # their bias + residual run on the large-tile kernel, as in the training forward
-            qkv = torch.addmm(w["bqkv16"], xa.view(M0, E), w["wqkv"].t()).view(nb, S0, 3, E)
-            if dt == torch.bfloat16 and rot > 0:   # rotate q,k once in place: cache fill becomes a copy, K3 runs its fast form
-                ops.rope_inplace(qkv.view(nb, S0, 3 * E)[:, :, :2 * E], 2 * H, rot, cos_t, sin_t)
-                rot = 0
-            ops.kv_cache_fill(qkv[:, :, 1], qkv[:, :, 2], kcs[li], vcs[li], H, rot, cos_t, sin_t)
-            a, _ = ops.prefix_attn_fwd(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], H, rot, P, cos_t, sin_t, layer.use_stablemax)
-            x = _lin(a.view(M0, E), w["wo"], w["bo"], res=x.view(M0, E), square=True).view(nb, S0, E)
-            xf, _, _ = ops.layernorm_fwd(x, layer.mlp_norm.weight, layer.mlp_norm.bias)
-            u = ops.relu2_fwd(torch.addmm(w["b116"], xf.view(M0, E), w["w1"].t()))     # fused on libmmhip it measured slower (prefill 27.5 vs 25 ms)
-            x = _lin(u, w["w2"], w["b2"], res=x.view(M0, E), square=True).view(nb, S0, E)  # prefill: N = E on the large-tile kernel
-
     use_graph = bool(graph)
     nsplit = _DECODE_SPLIT if (_DECODE_SPLIT > 1 and not use_graph and B >= 128 * _DECODE_SPLIT and B % _DECODE_SPLIT == 0) else 1
     n_done = 0
     # the prefill runs once for the whole batch (MFMA-bound: cutting it in two only made its products smaller -- measured
     # 741k against 753k tokens/s with the halves prefilled on their own streams)
-    prefill(prompt, cache.k, cache.v)
+    _prefill(dec, weights, prompt, Smax, lambda li, k, v, rot, cos_t, sin_t: ops.kv_cache_fill(k, v, cache.k[li], cache.v[li], H, rot, cos_t, sin_t))
     finished = torch.zeros(B, dtype=torch.bool, device=dev)
     # ---- decode steps
     def decode_step(cur, pos):
         """One token for every row: cur [B] ids at position pos-1 -> argmax ids at pos (pos: int, or int32 device scalar)."""
-        h = emb[cur].to(dt)                                                    # [B, E]
-        for li, layer in enumerate(dec.layers):
-            w = weights[li]
+        def attend(li, layer, qkv):
             cos_t, sin_t = layer.rotary_emb.half_tables(Smax)
-            # LN, QKV (+bias), K4, out-proj (+bias +residual fused), LN, W1 (+bias) relu^2, W2 (+bias) += residual; operands
-            # and bias copies come from the operand cache (no per-call casts)
-            xa, _, _ = ops.layernorm_fwd(h, layer.attn_norm.weight, layer.attn_norm.bias)
-            qkv = _lin(xa, w["wqkv"], w["bqkv"], w["bqkv16"])                  # [B, 3E]
-            a = ops.decode_attn(qkv[:, :E], qkv[:, E:2 * E], qkv[:, 2 * E:], cache.k[li], cache.v[li], H,
-                                layer.rotary_ndims, pos, cos_t, sin_t, layer.use_stablemax)
-            h = _lin(a, w["wo"], w["bo"], res=h, square=True)
-            xf, _, _ = ops.layernorm_fwd(h, layer.mlp_norm.weight, layer.mlp_norm.bias)
-            u = _lin(xf, w["w1"], w["b1"], w["b116"], act=ops.ACT_RELU2, square=True)      # libmmhip: bias + relu^2 fused
-            h = _lin(u, w["w2"], w["b2"], w["b216"], res=h)
-        xt, _, _ = ops.layernorm_fwd(h, dec.final_norm.weight, dec.final_norm.bias)
-        return ops.argmax_rows(_lin(xt, w_out, b_out, b_out16, out_dtype=torch.float32))
+            return ops.decode_attn(qkv[:, :E], qkv[:, E:2 * E], qkv[:, 2 * E:], cache.k[li], cache.v[li], H, layer.rotary_ndims, pos, cos_t,
+                                   sin_t, layer.use_stablemax)
+        return ops.argmax_rows(_rows_logits(dec, weights, emb[cur].to(dt), attend, w_out, b_out, b_out16))
 
     if use_graph and steps > 1:
         cur_s = torch.full((B,), bos_id, dtype=torch.long, device=dev)

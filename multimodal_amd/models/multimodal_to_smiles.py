@@ -24,10 +24,12 @@ class MultiModalToSMILESModel(nn.Module):
         return self.decoder(target_seq, memory, nmr_tokens)
 
     @th.no_grad()
-    def generate(self, nmr_tokens, ir_data, max_len=128, bos_id=12, eos_id=13, early_stop=True, graph=None):
+    def generate(self, nmr_tokens, ir_data, max_len=128, bos_id=12, eos_id=13, early_stop=True, graph=None, page_size=None, kv_budget=None,
+                 kv_recent=16):
         """Greedy decode with a KV cache; returns LongTensor [B, <=max_len+1] starting with BOS.  Token ids equal the
         reference loop's (train_autoregressive.py:80-116); rows keep emitting argmax ids after their EOS, as the
-        reference's `current_token` does -- cut with `multimodal_amd.generate.ids_to_strings`."""
+        reference's `current_token` does -- cut with `multimodal_amd.generate.ids_to_strings`.  page_size / kv_budget / kv_recent: a paged
+        cache, and one of bounded size (`multimodal_amd.generate.greedy_generate`)."""
         from ..generate import greedy_generate
         return greedy_generate(self, nmr_tokens, ir_data, max_len=max_len, bos_id=bos_id, eos_id=eos_id,
-                               early_stop=early_stop, graph=graph)
+                               early_stop=early_stop, graph=graph, page_size=page_size, kv_budget=kv_budget, kv_recent=kv_recent)

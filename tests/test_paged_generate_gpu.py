@@ -1,0 +1,141 @@
+"""Decoding over a paged cache: generate(page_size=...), a bounded cache (kv_budget), and drafted tokens (speculative_generate) against the
+dense cache's greedy loop.  float32: the paths add up the same products in other orders, so ids may differ only at near-ties; the
+models are random, their logits spread far wider than that, and the ids are required to be equal."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = torch.device("cuda", 0)
+
+
+def _model(seed, E=128, H=4, L=2, stablemax=False, max_seq=40):
+    from multimodal_amd.models import MultiModalToSMILESModel
+    torch.manual_seed(seed)
+    m = MultiModalToSMILESModel(591, 1000, max_seq_length=max_seq, max_nmr_length=16, max_memory_length=32, embed_dim=E, num_heads=H, num_layers=L,
+                                dropout=0.0, verbose=False, use_stablemax=stablemax).to(DEV)
+    with torch.no_grad():
+        m.decoder.out.weight.mul_(8)
+    return m.eval()
+
+
+def _inputs(B, seed=5):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(0, 1000, (B, 16), generator=g).to(DEV), torch.rand(B, 1000, generator=g).to(DEV)
+
+
+@pytest.fixture(autouse=True)
+def _float32():
+    import multimodal_amd as mm
+    with mm.compute_dtype(torch.float32):
+        yield
+
+
+@pytest.mark.parametrize("stablemax", [False, True])
+@pytest.mark.parametrize("page", [4, 16, 64])
+def test_paged_ids_are_the_dense_ids(page, stablemax):
+    m = _model(1, stablemax=stablemax)
+    nmr, ir = _inputs(6)
+    want = m.generate(nmr, ir, max_len=30, early_stop=False)
+    assert torch.equal(m.generate(nmr, ir, max_len=30, early_stop=False, page_size=page), want)
+    # a budget that nothing exceeds changes nothing
+    assert torch.equal(m.generate(nmr, ir, max_len=30, early_stop=False, page_size=page, kv_budget=200), want)
+
+
+def test_paged_bf16_runs_and_stays_close():
+    import multimodal_amd as mm
+    m = _model(2)
+    nmr, ir = _inputs(8)
+    with mm.compute_dtype(torch.bfloat16):
+        a, b = m.generate(nmr, ir, max_len=20, early_stop=False), m.generate(nmr, ir, max_len=20, early_stop=False, page_size=16)
+    assert torch.equal(a[:, :2], b[:, :2])                                     # later ids may part at bf16 near-ties
+
+
+def test_budget_bounds_the_cache_and_keeps_what_comes_before_the_first_eviction():
+    from multimodal_amd import generate as G
+    m = _model(3)
+    nmr, ir = _inputs(5)
+    want = m.generate(nmr, ir, max_len=36, early_stop=False)
+    made, evicted = [], []
+    init, evict = G.PagedKVCache.__init__, G.PagedKVCache.evict
+
+    def spy_init(self, *a, **k):
+        init(self, *a, **k)
+        made.append(self)
+
+    def spy_evict(self, budget, recent):
+        evict(self, budget, recent)
+        evicted.append(self.lengths.tolist())
+    G.PagedKVCache.__init__, G.PagedKVCache.evict = spy_init, spy_evict
+    try:
+        got = m.generate(nmr, ir, max_len=36, early_stop=False, page_size=8, kv_budget=30, kv_recent=6)
+    finally:
+        G.PagedKVCache.__init__, G.PagedKVCache.evict = init, evict
+    P = 31 + 16                                                                # memory and NMR tokens
+    assert made[0].page_table.shape[1] * 8 < P + 6 + 8                         # not P + 36 slots
+    assert len(evicted) >= 5 and all(n == [30] * 5 for n in evicted)
+    assert torch.equal(got[:, :7], want[:, :7]) and got.shape == want.shape
+    assert ((got >= 0) & (got < 591)).all()
+
+
+def test_budget_arguments():
+    m = _model(3)
+    nmr, ir = _inputs(2)
+    for kw in (dict(kv_budget=8, kv_recent=9), dict(kv_budget=8, kv_recent=0), dict(page_size=16, graph=True)):
+        with pytest.raises(ValueError):
+            m.generate(nmr, ir, max_len=4, **kw)
+    with pytest.raises(RuntimeError, match="power of two"):
+        m.generate(nmr, ir, max_len=4, page_size=12)
+
+
+def _cut(ids, eos):
+    out = []
+    for row in ids.tolist():
+        out.append(row[: row.index(eos, 1) + 1] if eos in row[1:] else row)
+    return out
+
+
+@pytest.mark.parametrize("n_draft", [1, 3, 6])
+@pytest.mark.parametrize("same", [True, False])
+def test_drafted_greedy_ids_are_the_greedy_ids(same, n_draft):
+    """temperature = 0: whatever the draft proposes, the ids are the model's own; with a draft of its own weights all are accepted."""
+    from multimodal_amd import ops
+    from multimodal_amd.generate import speculative_generate
+    m, d = _model(7), _model(7 if same else 8, E=128 if same else 64, L=2 if same else 1)
+    nmr, ir = _inputs(7)
+    want = m.generate(nmr, ir, max_len=25, early_stop=False)
+    eos = int(want[2, 9])                                                      # an id that does occur ends some rows early
+    counts, orig = [], ops.verify_drafts
+
+    def spy(drafts, *a, **k):
+        r = orig(drafts, *a, **k)
+        if drafts.shape[1]:
+            counts.append(r[1].tolist())
+        return r
+    ops.verify_drafts = spy
+    try:
+        got = speculative_generate(m, d, nmr, ir, max_len=25, eos_id=eos, pad_id=0, n_draft=n_draft, temperature=0)
+    finally:
+        ops.verify_drafts = orig
+    for row, full in zip(got.tolist(), _cut(want, eos)):
+        assert row[: len(full)] == full[: len(row)] and all(x == 0 for x in row[len(full):])
+    if same:
+        assert all(x == n_draft for x in counts[0])
+
+
+def test_drafted_samples_are_repeatable_and_valid():
+    from multimodal_amd.generate import speculative_generate
+    m, d = _model(9), _model(10, E=64, L=1)
+    nmr, ir = _inputs(9)
+    run = lambda seed: speculative_generate(m, d, nmr, ir, max_len=20, n_draft=3, temperature=1.3, generator=torch.Generator(device=DEV).manual_seed(seed))
+    a, b, c = run(1), run(1), run(2)
+    assert torch.equal(a, b) and (a.shape != c.shape or not torch.equal(a, c))
+    assert (a[:, 0] == 12).all() and a.shape[1] <= 21 and ((a >= 0) & (a < 591)).all()
+
+
+def test_drafting_refuses():
+    from multimodal_amd.generate import speculative_generate
+    m = _model(9)
+    nmr, ir = _inputs(2)
+    for kw in (dict(n_draft=0), dict(temperature=-1.0)):
+        with pytest.raises(ValueError):
+            speculative_generate(m, m, nmr, ir, **kw)

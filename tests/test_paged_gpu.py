@@ -308,6 +308,54 @@ def test_long_rows_beside_short_ones(dtype):
     _check_step(c, before, q, k, v, lens, 2, 64, tabs, False, None, o)
 
 
+@pytest.mark.parametrize("dtype,G,d,width,weights", [
+    (torch.bfloat16, 1, 64, 0, False), (torch.bfloat16, 4, 36, 0, True), (torch.float32, 2, 64, 0, False), (torch.bfloat16, 3, 128, 32, False),
+    (torch.float32, 1, 100, 32, True), (torch.bfloat16, 8, 64, 32, False), (torch.bfloat16, 1, 512, 32, False), (torch.float32, 1, 512, 32, False)])
+def test_many_short_rows(dtype, G, d, width, weights):
+    """More rows and heads than the card has waves, of 0 to 60 slots: a wave each (up to four query heads a KV head).  width = 32: tables as wide
+    as 512 slots, a cache too large for the last-level cache by what it could hold.  A few rows against the definition, all of them against
+    a call of their own."""
+    from multimodal_amd import ops
+    B, Hkv, rot = 512, 4, d // 4 * 2
+    g = torch.Generator().manual_seed(14)
+    lens = torch.randint(-1, 61, (B,), generator=g).tolist()
+    c, q, k, v = _filled(14, dtype, B, Hkv, G, d, 16, lens, weights=weights)
+    if width:
+        c.table = torch.nn.functional.pad(c.table, (0, width - c.table.shape[1]), value=-1).contiguous()
+    before = (c.k.clone(), c.v.clone(), None if c.w is None else c.w.clone())
+    tabs = _tables(rot, 61)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = ops.paged_decode_attn(q, k, v, c.k, c.v, c.table, n, Hkv * G, rot, *tabs, False, weights=c.w)
+    few = list(range(0, B, 37))
+    sub = Cache.__new__(Cache)
+    sub.__dict__.update(c.__dict__)
+    sub.table = c.table[few].contiguous()
+    # what the other rows did to their own pages is theirs: the check of untouched slots takes it as given
+    mine = torch.zeros(c.n_pages, dtype=torch.bool, device=DEV)
+    mine[sub.table[sub.table >= 0].long()] = True
+    base = tuple(None if x is None else torch.where(mine.view(-1, *[1] * (x.dim() - 1)), x, y) for x, y in zip(before, (c.k, c.v, c.w)))
+    _check_step(sub, base, q[few], k[few], v[few], [lens[b] for b in few], Hkv * G, rot, tabs, False, None, o[few])
+    for i in range(0, B, 64):
+        s = slice(i, i + 64)
+        part = ops.paged_decode_attn(q[s], None, None, c.k, c.v, c.table[s], torch.where(n[s] < 0, n[s], n[s] + 1), Hkv * G, rot, *tabs, False)
+        # two evaluations of the same stored slots: each within the bound, whose sum part is below 2^-12 of the largest value here
+        assert ((part.float() - o[s].float()).abs() <= 2 * HALF[dtype] * o[s].float().abs() + 2.0 ** -12 * float(o.float().abs().max())).all(), i
+
+
+def test_tables_far_wider_than_the_rows():
+    """A table of 200000 slots for rows of a few: splits beyond a row's end do nothing."""
+    from multimodal_amd import ops
+    for dtype in (torch.bfloat16, torch.float32):
+        lens = [700, 3, 0, -1]
+        c, q, k, v = _filled(15, dtype, 4, 2, 2, 64, 32, lens, weights=True)
+        c.table = torch.nn.functional.pad(c.table, (0, 6250 - c.table.shape[1]), value=-1).contiguous()
+        before = (c.k.clone(), c.v.clone(), c.w.clone())
+        n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+        o = ops.paged_decode_attn(q, k, v, c.k, c.v, c.table, n, 4, 0, None, None, False, weights=c.w)
+        c.table = c.table[:, :40].contiguous()
+        _check_step(c, before, q, k, v, lens, 4, 0, (None, None), False, None, o)
+
+
 def test_offsets_past_32_bits():
     """A pool of more than 2^32 bytes and 2^31 elements: pages at its end (store, attend, fill, evict)."""
     from multimodal_amd import ops
@@ -493,6 +541,10 @@ EVICT = [
     (torch.bfloat16, 1, 512, 32, [3500, 2049], 2048, 7),
     (torch.bfloat16, 2, 64, 16, [50, 60], 100, 10),
     (torch.float32, 2, 64, 128, [20000, 16384, 9000], 8000, 900),
+    (torch.bfloat16, 1, 8, 1024, [70000, 66000, 5], 30000, 1000),              # more slots than a workgroup's registers hold
+    (torch.bfloat16, 1, 12, 256, [40000, 33000], 32000, 31000),                # a long shift that overlaps itself
+    (torch.bfloat16, 2, 128, 16, [4000, 2100], 2000, 0),
+    (torch.float32, 1, 128, 64, [3001, 3002], 3000, 2999),
 ]
 
 
