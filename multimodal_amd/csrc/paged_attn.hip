@@ -22,6 +22,9 @@
 
 typedef __attribute__((ext_vector_type(4))) unsigned u4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned u2_t;
+typedef u4_t __attribute__((aligned(8))) u4_8_t;
+typedef u4_t __attribute__((aligned(2))) u4_2_t;                    // rows of q and the new key need no alignment beyond a value's
+typedef f32x4_t __attribute__((aligned(4))) f4_4_t;
 
 struct PagedP {
     const void* q; const void* kn; const void* vn; void* kpool; void* vpool; void* o; float* w; const int* lengths; const int* positions;
@@ -35,14 +38,49 @@ __device__ __forceinline__ int paged_pos(const int* positions, const int* length
     const int pos = positions ? positions[b] : (append ? n : n - 1);
     return min(max(pos, 0), n_pos - 1);
 }
-// element c of a head, rotated (half layout over the first rot dims) at the table row cs / sn
-template <typename T> __device__ __forceinline__ float rotated(const T* x, int c, int rot, const float* cs, const float* sn) {
+// values c .. c + 7 (bf16) or c + 3 (f32) of a row of d, 0 past its end
+__device__ __forceinline__ void raw_piece(const bf16* x, int c, int d, float (&v)[8]) {
+    if (c + 8 <= d) {
+        const u4_t w = *reinterpret_cast<const u4_2_t*>(x + c);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+    } else
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = c + i < d ? to_f(x[c + i]) : 0.f;
+}
+__device__ __forceinline__ void raw_piece(const float* x, int c, int d, float (&v)[4]) {
+    const f32x4_t w = c < d ? *reinterpret_cast<const f4_4_t*>(x + c) : f32x4_t{0.f, 0.f, 0.f, 0.f};    // d % 4 == 0
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = w[i];
+}
+// the same, rotated (half layout over the first rot values) at the table row cs / sn
+template <typename T, int PE> __device__ __forceinline__ void piece(const T* x, int c, int d, int rot, const float* cs, const float* sn, float (&v)[PE]) {
+    raw_piece(x, c, d, v);
+    if (c >= rot) return;
     const int half = rot >> 1;
-    const float a = to_f(x[c]);
-    if (c >= rot) return a;
-    const int i = c < half ? c : c - half;
-    const float o = to_f(x[c < half ? c + half : c - half]);
-    return c < half ? fmaf(a, cs[i], -(o * sn[i])) : fmaf(a, cs[i], o * sn[i]);
+    if (half % PE == 0) {
+        const bool low = c < half;
+        const int i = low ? c : c - half;
+        float o[PE], cv[PE], sv[PE];
+        raw_piece(x, low ? c + half : i, d, o);
+#pragma unroll
+        for (int e = 0; e < PE; e += 4) {
+            const f32x4_t a = *reinterpret_cast<const f4_4_t*>(cs + i + e), b = *reinterpret_cast<const f4_4_t*>(sn + i + e);
+#pragma unroll
+            for (int k = 0; k < 4; k++) { cv[e + k] = a[k]; sv[e + k] = b[k]; }
+        }
+#pragma unroll
+        for (int e = 0; e < PE; e++) v[e] = low ? fmaf(v[e], cv[e], -(o[e] * sv[e])) : fmaf(v[e], cv[e], o[e] * sv[e]);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < PE; e++)
+        if (c + e < rot) {
+            const bool low = c + e < half;
+            const int i = low ? c + e : c + e - half;
+            const float o = to_f(x[low ? c + e + half : i]);
+            v[e] = low ? fmaf(v[e], cs[i], -(o * sn[i])) : fmaf(v[e], cs[i], o * sn[i]);
+        }
 }
 // stablemax's s(x); the reciprocal is within one unit in the last place
 __device__ __forceinline__ float stable_s(float x) { return x < 0.f ? __builtin_amdgcn_rcpf(1.f - x + 1e-9f) : x + 1.f; }
@@ -67,10 +105,10 @@ __device__ __forceinline__ void lds_barrier() {
 }
 
 // ------------------------------------------------------------------------------------------------ operands of one step (16 NT slots)
-// VE: columns a lane loads of a V row (16 lanes x VE = one slab), NS: slabs of a head, NT: tiles of 16 slots in a step, AL8: rows are
-// multiples of 8 values (16-byte pieces).  K of the whole step is in registers; of V up to two slabs, the others follow as those are used
+// VE: columns a lane loads of a V row (16 lanes x VE = one slab), NS: slabs of a head, NT: tiles of 16 slots in a step, AL: what a row of K
+// is made of: 2 = whole 16-byte pieces, 1 = 8-byte pieces, 0 = one 8-byte piece.  K of the whole step is in registers; of V up to two slabs, the others follow as those are used
 // up (a head of 512 would need 512 registers for its step otherwise).
-template <typename T, int VE_, int NS_, int NT_, bool AL8, bool ST> struct Step {
+template <typename T, int VE_, int NS_, int NT_, int AL, bool ST> struct Step {
     static constexpr bool BF = std::is_same<T, bf16>::value;
     static constexpr int VE = VE_, NS = NS_, NT = NT_, J = 4 * NT, DP = 16 * VE * NS;
     static constexpr int PE = BF ? 8 : 4, CW = 4 * PE, KC = DP / CW;           // values in a lane's piece of K, columns of a matrix instruction
@@ -92,12 +130,9 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8, bool ST> struct Step 
 #pragma unroll
             for (int c = 0; c < KC; c++) {
                 const int col = c * CW + g * PE;
-                if constexpr (AL8) {
-                    k[t][c] = read<u4_t>(r + (col < d ? col : 0));
-                } else {
-                    const u2_t a = read<u2_t>(r + (col < d ? col : 0)), b = read<u2_t>(r + (col + 4 < d ? col + 4 : 0));
-                    k[t][c] = u4_t{a[0], a[1], b[0], b[1]};
-                }
+                if constexpr (AL == 2) k[t][c] = read<u4_t>(r + (col < d ? col : 0));
+                else if constexpr (AL == 1) k[t][c] = read<u4_8_t>(r + min(col, d - 8));      // the last half piece: trim_k takes it from the end
+                else { const u2_t a = read<u2_t>(r); k[t][c] = u4_t{a[0], a[1], 0u, 0u}; }
             }
         }
     }
@@ -110,7 +145,7 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8, bool ST> struct Step 
 #pragma unroll
                 for (int t = 0; t < NT; t++) {
                     if (col >= d) k[t][c] = u4_t{0u, 0u, 0u, 0u};
-                    else if (!AL8 && col + 4 >= d) { k[t][c][2] = 0u; k[t][c][3] = 0u; }
+                    else if (AL == 1 && col + 4 >= d) k[t][c] = u4_t{k[t][c][2], k[t][c][3], 0u, 0u};
                 }
             }
     }
@@ -135,16 +170,26 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8, bool ST> struct Step 
 #pragma unroll
             for (int c = 0; c < KC; c++) k[0][c] = *reinterpret_cast<const u4_t*>(ks + c * CW + g * PE);
     }
-    // value (head, column) of q, as QT terms: rows [term][heads]
-    static __device__ __forceinline__ void put_q(T* lds, int heads, int head, int c, float x) {
+    // piece c .. c + PE - 1 of a head's q, as QT terms: rows [term][heads]
+    static __device__ __forceinline__ void put_q(T* lds, int heads, int head, int c, float (&x)[PE]) {
         T* f = lds + head * QS + c;
-        if constexpr (!BF) { *f = x; return; }
-        const float least = x == 0.f ? 0.f : copysignf(0x1p-100f, x);
+        if constexpr (!BF) { *reinterpret_cast<f32x4_t*>(f) = f32x4_t{x[0], x[1], x[2], x[3]}; }
+        else {
+            float least[PE];
 #pragma unroll
-        for (int t = 0; t < QT; t++) {
-            const float h = __uint_as_float(__float_as_uint(x) & 0xffff0000u);
-            f[t * heads * QS] = from_f<T>(t && h == 0.f ? least : h);
-            x -= h;
+            for (int e = 0; e < PE; e++) least[e] = x[e] == 0.f ? 0.f : copysignf(0x1p-100f, x[e]);
+#pragma unroll
+            for (int t = 0; t < QT; t++) {
+                unsigned w[PE];
+#pragma unroll
+                for (int e = 0; e < PE; e++) {
+                    const float h = __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
+                    w[e] = __float_as_uint(t && h == 0.f ? least[e] : h);
+                    x[e] -= h;
+                }
+                *reinterpret_cast<u4_t*>(f + t * heads * QS) =
+                    u4_t{w[0] >> 16 | w[1], w[2] >> 16 | w[3], w[4] >> 16 | w[5], w[6] >> 16 | w[7]};
+            }
         }
     }
     // the scores of the step's tiles; q: this lane's head and piece in LDS.  Columns that are not rotated are exact in q's first term.
@@ -244,9 +289,9 @@ template <typename T, int VE_, int NS_, int NT_, bool AL8, bool ST> struct Step 
 // ------------------------------------------------------------------------------------------------ the walk
 // WPR: waves that share a (row, KV head, split): 4 (merged through LDS), or 1 (four of them side by side in a workgroup).  ST: the cache is
 // read past the last-level cache (non-temporal).
-template <typename T, int VE, int NS, int NT, bool AL8, int WPR, bool ST>
+template <typename T, int VE, int NS, int NT, int AL, int WPR, bool ST>
 __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS * sizeof(T) * NT <= 48 ? 2 : 1)) void paged_attn_k(const PagedP p) {
-    typedef Step<T, VE, NS, NT, AL8, ST> S_t;
+    typedef Step<T, VE, NS, NT, AL, ST> S_t;
     constexpr int SW = 16 * VE, DP = SW * NS, SL = 16 * NT, RD = WPR * SL, J = 4 * NT;    // a wave's step, a round of the waves of a row
     constexpr int HEADS = WPR == 4 ? 16 : 4, QB = S_t::QT * HEADS * S_t::QS * (int)sizeof(T);   // query heads a tile may have (launch)
     constexpr int MERGE = WPR == 4 ? 4 * 16 * SW * 4 : 0, TEAMS = 4 / WPR, TT = 64 * WPR;
@@ -322,21 +367,29 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
     // ---- q (and the new key), rotated, while the first rows are under way
     const long trow = (long)paged_pos(p.positions, p.lengths, p.kn != nullptr, p.n_pos, b) * (p.rot >> 1);
     const float* cs = p.cos_t + trow; const float* sn = p.sin_t + trow;
-    if (d < DP) {                                                                       // columns past d: zero, as in trim_k
-        const int pad = DP - d;
-        for (int i = tid; i < nh * pad; i += TT) S_t::put_q(qlds, HEADS, i / pad, d + i % pad, 0.f);
-        if (mine) for (int c = d + tid; c < DP; c += TT) own_k[c] = own_v[c] = from_f<T>(0.f);
-    }
-    for (int i = tid; i < nh * d; i += TT) {
-        const int h = i / d, c = i - h * d;
-        S_t::put_q(qlds, HEADS, h, c, rotated((const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d, c, p.rot, cs, sn));
+    constexpr int PE = S_t::PE, PIECES = DP / PE;                                       // columns past d: zero, as in trim_k
+    for (int i = tid; i < nh * PIECES; i += TT) {
+        const int h = i / PIECES, c = i % PIECES * PE;
+        float x[PE];
+        piece((const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d, c, d, p.rot, cs, sn, x);
+        S_t::put_q(qlds, HEADS, h, c, x);
     }
     if (mine)
-        for (int c = tid; c < d; c += TT) {
-            const T kv = from_f<T>(rotated((const T*)p.kn + (long)b * p.ld_k + (long)hk * d, c, p.rot, cs, sn));
-            const T vv = ((const T*)p.vn)[(long)b * p.ld_v + (long)hk * d + c];
-            own_k[c] = kv; own_v[c] = vv;
-            if (own_row >= 0 && ct == 0) { ((T*)p.kpool)[own_row * d + c] = kv; ((T*)p.vpool)[own_row * d + c] = vv; }
+        for (int i = tid; i < PIECES; i += TT) {
+            const int c = i * PE;
+            float x[PE], y[PE];
+            piece((const T*)p.kn + (long)b * p.ld_k + (long)hk * d, c, d, p.rot, cs, sn, x);
+            raw_piece((const T*)p.vn + (long)b * p.ld_v + (long)hk * d, c, d, y);
+            VecIO<T, PE>::store(own_k + c, x); VecIO<T, PE>::store(own_v + c, y);       // the key rounded to the cache's type, as it is stored
+            if (own_row >= 0 && ct == 0) {
+                T* kd = (T*)p.kpool + own_row * d + c; T* vd = (T*)p.vpool + own_row * d + c;
+#pragma unroll
+                for (int e = 0; e < PE; e += 4)
+                    if (c + e < d) {
+                        const float a[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]}, w[4] = {y[e], y[e + 1], y[e + 2], y[e + 3]};
+                        VecIO<T, 4>::store(kd + e, a); VecIO<T, 4>::store(vd + e, w);
+                    }
+            }
         }
     sync();
     const T* q = qlds + min(li, nh - 1) * S_t::QS + g * S_t::PE;                        // columns past the last head repeat it; nothing reads them
@@ -591,8 +644,8 @@ extern "C" size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* a) {
     return r.part + r.stat + r.sc;
 }
 
-template <typename T, int VE, int NS, int NT, bool AL8> static void paged_launch(const PagedP& p, bool lone, bool past, hipStream_t st) {
-#define MM_PAGED(WPR_, ST_) hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL8, WPR_, ST_>), dim3((unsigned)cdiv(p.units, WPR_ == 1 ? 4 : 1)), dim3(256), 0, st, p)
+template <typename T, int VE, int NS, int NT, int AL> static void paged_launch(const PagedP& p, bool lone, bool past, hipStream_t st) {
+#define MM_PAGED(WPR_, ST_) hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL, WPR_, ST_>), dim3((unsigned)cdiv(p.units, WPR_ == 1 ? 4 : 1)), dim3(256), 0, st, p)
     if (lone) { if (past) MM_PAGED(1, true); else MM_PAGED(1, false); }
     else { if (past) MM_PAGED(4, true); else MM_PAGED(4, false); }
 #undef MM_PAGED
@@ -636,23 +689,24 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     const bool past = a->B * a->Hkv * a->width * a->page * a->d * (a->dtype == MM_BF16 ? 4 : 8) > (256LL << 20);
     const int64_t d = a->d;
     if (a->dtype == MM_F32) {
-        if (d <= 64) paged_launch<float, 4, 1, 1, true>(p, lone, past, st);
-        else if (d <= 128) paged_launch<float, 4, 2, 1, true>(p, lone, past, st);
-        else if (d <= 192) paged_launch<float, 4, 3, 1, true>(p, lone, past, st);
-        else if (d <= 256) paged_launch<float, 4, 4, 1, true>(p, lone, past, st);
-        else paged_launch<float, 4, 8, 1, true>(p, lone, past, st);
+        if (d <= 64) paged_launch<float, 4, 1, 1, 2>(p, lone, past, st);
+        else if (d <= 128) paged_launch<float, 4, 2, 1, 2>(p, lone, past, st);
+        else if (d <= 192) paged_launch<float, 4, 3, 1, 2>(p, lone, past, st);
+        else if (d <= 256) paged_launch<float, 4, 4, 1, 2>(p, lone, past, st);
+        else paged_launch<float, 4, 8, 1, 2>(p, lone, past, st);
     } else if (d % 8 == 0) {
-        if (d <= 64) paged_launch<bf16, 4, 1, 2, true>(p, lone, past, st);
-        else if (d <= 128) paged_launch<bf16, 8, 1, 2, true>(p, lone, past, st);
-        else if (d <= 192) paged_launch<bf16, 4, 3, 2, true>(p, lone, past, st);
-        else if (d <= 256) paged_launch<bf16, 8, 2, 2, true>(p, lone, past, st);
-        else paged_launch<bf16, 8, 4, 1, true>(p, lone, past, st);
+        if (d <= 64) paged_launch<bf16, 4, 1, 2, 2>(p, lone, past, st);
+        else if (d <= 128) paged_launch<bf16, 8, 1, 2, 2>(p, lone, past, st);
+        else if (d <= 192) paged_launch<bf16, 4, 3, 2, 2>(p, lone, past, st);
+        else if (d <= 256) paged_launch<bf16, 8, 2, 2, 2>(p, lone, past, st);
+        else paged_launch<bf16, 8, 4, 1, 2>(p, lone, past, st);
     } else {                                                                            // rows of whole 8-byte pieces only
-        if (d <= 64) paged_launch<bf16, 4, 1, 2, false>(p, lone, past, st);
-        else if (d <= 128) paged_launch<bf16, 4, 2, 2, false>(p, lone, past, st);
-        else if (d <= 192) paged_launch<bf16, 4, 3, 2, false>(p, lone, past, st);
-        else if (d <= 256) paged_launch<bf16, 4, 4, 2, false>(p, lone, past, st);
-        else paged_launch<bf16, 4, 8, 1, false>(p, lone, past, st);
+        if (d == 4) paged_launch<bf16, 4, 1, 2, 0>(p, lone, past, st);
+        else if (d <= 64) paged_launch<bf16, 4, 1, 2, 1>(p, lone, past, st);
+        else if (d <= 128) paged_launch<bf16, 4, 2, 2, 1>(p, lone, past, st);
+        else if (d <= 192) paged_launch<bf16, 4, 3, 2, 1>(p, lone, past, st);
+        else if (d <= 256) paged_launch<bf16, 4, 4, 2, 1>(p, lone, past, st);
+        else paged_launch<bf16, 4, 8, 1, 1>(p, lone, past, st);
     }
     MM_LAUNCH_CHECK();
     if (blocks2) {

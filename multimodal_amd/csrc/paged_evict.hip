@@ -60,10 +60,7 @@ template <int NW, int R> __device__ __forceinline__ void evict_select(const Evic
     int* kept = p.kept + bh * p.budget;
     int* hd = p.head(bh);
     if (tid == 0) { hd[0] = n; hd[1] = 0; }
-    if (n <= p.budget) {
-        for (int j = tid; j < p.budget; j += NW * 64) kept[j] = j < n ? j : -1;
-        return;
-    }
+    if (n <= p.budget) return;
     const int A = p.budget - p.recent, old = n - p.recent, rounds = (old + ROUND - 1) / ROUND;
     // the moves as slots: in LDS where they fit (at most half of the slots move)
     constexpr int LIST = R > 0 && NW * R * 64 <= 8192 ? NW * R * 32 : 0;
@@ -248,10 +245,14 @@ template <typename U> __device__ __forceinline__ void evict_shift(const EvictP& 
 }
 
 // ------------------------------------------------------------------------------------------------ kernels
-// ALL: select, move and shift in one workgroup per (row, KV head); else the selection alone
+// A workgroup per (row, KV head).  ALL: it moves and shifts as well.
 template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW * 64) void evict_select_k(const EvictP p) {
     __shared__ int red[2 * NW];
-    const int b = blockIdx.x, h = blockIdx.y;
+    const int b = blockIdx.x, h = blockIdx.y, n = min(p.lengths[b], p.map.capacity());
+    if (n <= p.budget) {
+        int* kept = p.kept + ((long)b * p.map.Hkv + h) * p.budget;
+        for (int j = threadIdx.x; j < p.budget; j += NW * 64) kept[j] = j < n ? j : -1;
+    }
     evict_select<NW, R>(p, b, h, red);
     if constexpr (ALL) {
         __syncthreads();
@@ -290,9 +291,9 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
     // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 181 in three).
     const bool all = ((int64_t)p.room + p.recent) * p.units <= 8192;
 #define MM_SELECT(NW_, R_) do { if (all) hipLaunchKernelGGL((evict_select_k<NW_, R_, U, true>), grid, dim3(NW_ * 64), 0, st, p); \
-                                else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
-    if (cap <= 1024) MM_SELECT(4, 4);                                          // eight waves: fewer share a barrier's price (8192 slots: 26 us, 16 waves 37, 4 waves 33)
-    else if (cap <= 8192) MM_SELECT(8, 16);
+                                     else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
+    if (cap <= 1024) MM_SELECT(4, 4);
+    else if (cap <= 8192) MM_SELECT(8, 16);                               // eight waves: 26 us for 384 heads of 8192 slots, 16 waves 37, four 33
     else if (cap <= 32768) MM_SELECT(8, 64);
     else if (cap <= 65536) MM_SELECT(8, 128);
     else MM_SELECT(16, 0);
