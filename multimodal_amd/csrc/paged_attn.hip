@@ -33,6 +33,17 @@ struct PagedP {
     int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, units, stable; long ld_q, ld_k, ld_v; float scale;
 };
 
+// Slots of row b that the call attends over (its own token among them), and how they are split: into ceil(cover / chunk) even parts, in whole
+// rounds of 128 slots.
+__device__ __forceinline__ int paged_cover(const PagedP& p, int len) {
+    const int cap = p.map.capacity();
+    return len < 0 ? 0 : min(min(len, cap) + (p.kn ? 1 : 0), cap);
+}
+__device__ __forceinline__ int paged_part(const PagedP& p, int cover) {
+    const int ns = max(1, (cover + p.chunk - 1) / p.chunk);
+    return max(128, ((cover + ns - 1) / ns + 127) & ~127);
+}
+
 __device__ __forceinline__ int paged_pos(const int* positions, const int* lengths, bool append, int n_pos, int b) {
     const int n = lengths[b];
     const int pos = positions ? positions[b] : (append ? n : n - 1);
@@ -308,16 +319,20 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
     };
     unsigned id = blockIdx.x * TEAMS + team;
     if (WPR == 1 && id >= (unsigned)p.units) return;
-    const int split = (int)(id % (unsigned)p.nsplit); id /= (unsigned)p.nsplit;
+    // An odd number of workgroups a tile: they go round the eight XCDs, and with an even one those of the splits that short rows do not have stood
+    // idle (452 rows and heads of 360 to 857 slots in up to two splits: 51 us; 40).
+    const unsigned step = (unsigned)p.nsplit | 1u;
+    const int split = (int)(id % step); id /= step;
+    if (split >= p.nsplit) return;
     const int ct = (int)(id % (unsigned)p.ctiles); id /= (unsigned)p.ctiles;
     const int hk = (int)(id % (unsigned)p.Hkv), b = (int)(id / (unsigned)p.Hkv);
     const int d = p.d, cap = p.map.capacity(), len = p.lengths[b];
     const int h0 = hk * p.G + ct * 16, nh = min(16, p.G - ct * 16);                     // this tile's query heads
     const int n = min(max(len, 0), cap);                                                // slots in the cache
-    const int cover = len < 0 ? 0 : min(n + (p.kn ? 1 : 0), cap);
-    const int lo = split * p.chunk, hi = min(n, lo + p.chunk);
+    const int cover = paged_cover(p, len), part = paged_part(p, cover);
+    const int lo = split * part, hi = min(n, lo + part);
     if (split && lo >= cover) return;
-    const bool mine = p.kn && len >= 0 && len < cap && len >= lo && len < lo + p.chunk; // the new token falls into this split
+    const bool mine = p.kn && len >= 0 && len < cap && len >= lo && len < lo + part;    // the new token falls into this split
     const long own_row = mine ? p.map.row(b, hk, len) : -1;
     const T* kp = (const T*)p.kpool; const T* vp = (const T*)p.vpool;
     const int shift = p.map.shift, mask = (1 << shift) - 1;
@@ -528,10 +543,6 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
 }
 
 // ------------------------------------------------------------------------------------------------ joining the splits, adding the weights up
-__device__ __forceinline__ int paged_cover(const PagedP& p, int b) {
-    const int len = p.lengths[b], cap = p.map.capacity();
-    return len < 0 ? 0 : min(min(len, cap) + (p.kn ? 1 : 0), cap);
-}
 // Final maximum and 1 / sum of a head over its splits, by one wave (lanes take the splits in turn): every lane gets them.
 __device__ __forceinline__ void paged_final(const PagedP& p, long bh, int ns, float& base, float& inv) {
     const int lane = threadIdx.x & 63;
@@ -556,16 +567,16 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
     if ((int)blockIdx.x < joins) {
         const int bh = blockIdx.x, b = bh / p.H, cols = p.d >> 2, per = NTH / cols;
         const int c = tid % cols, gr = tid / cols;
-        const int ns = (paged_cover(p, b) + p.chunk - 1) / p.chunk;
+        const int cover = paged_cover(p, p.lengths[b]), part = paged_part(p, cover), ns = (cover + part - 1) / part;
         float base, inv;
         paged_final(p, bh, ns, base, inv);
         const float2* st = p.stat + (long)bh * p.nsplit;
-        const float* part = p.part + (long)bh * p.nsplit * p.d + c * 4;
+        const float* from = p.part + (long)bh * p.nsplit * p.d + c * 4;
         f32x4_t a = {0.f, 0.f, 0.f, 0.f};
         if (gr < per) {
 #pragma unroll 4
             for (int s = gr; s < ns; s += per)
-                a += *reinterpret_cast<const f32x4_t*>(part + (long)s * p.d) * (p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base));
+                a += *reinterpret_cast<const f32x4_t*>(from + (long)s * p.d) * (p.stable ? 1.f : __builtin_amdgcn_exp2f(st[s].x - base));
         }
         *reinterpret_cast<f32x4_t*>(red + tid * 4) = a;
         __syncthreads();
@@ -577,9 +588,9 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
         return;
     }
     const int id = blockIdx.x - joins, ch = id % wchunks, bk = id / wchunks, b = bk / p.Hkv, hk = bk % p.Hkv;
-    const int n = paged_cover(p, b), s0 = ch * (NTH * 4);
+    const int len = p.lengths[b], n = paged_cover(p, len), s0 = ch * (NTH * 4);
     if (s0 >= n) return;
-    const int ns = (n + p.chunk - 1) / p.chunk, cap = p.map.capacity();
+    const int part = paged_part(p, n), ns = (n + part - 1) / part, cap = p.map.capacity();
     const int slot = s0 + tid * 4;
     const long row = slot < n ? p.map.row(b, hk, slot) : -1;                            // four slots of one page (page >= 4)
     f32x4_t old = {0.f, 0.f, 0.f, 0.f}, add = old;
@@ -603,7 +614,6 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
             }
     }
     if (row < 0) return;
-    const int len = p.lengths[b];
     if (slot + 4 <= n && !(p.kn && slot + 4 > len)) {
         *reinterpret_cast<f32x4_t*>(p.w + row) = old + add;
     } else {
@@ -613,14 +623,15 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
     }
 }
 
-// How a cache of `cap` slots is split, in whole rounds of 128: up to 512 slots not at all (a second launch costs more than it saves: 24.7 us
-// against 33.5 for 32 rows of 16 heads and 500 slots), else so that there are about 512 workgroups (1 row of 65551 slots, 4 KV heads: 38 us,
-// 44 with four times as many), and in parts of at most 1024 slots, which even out rows of different lengths (32 rows of 300 to 16384
-// slots, 8 KV heads: 249 us; 263 in parts of 512, whose outputs are twice as many).
+// The most slots of a part, a whole number of rounds of 128.  Not split: up to 512 slots (a second launch costs more than it saves: 24.7 us
+// against 33.5 for 32 rows of 16 heads and 500 slots), and up to 2048 where there are rows and heads for more than one workgroup a CU (512
+// of 1000 to 2000 slots: 75 us, 84 in two parts; 452 heads of 256 and up to 857: 67, 78).  Else parts for about 768 workgroups (16 rows
+// of up to 3000 slots, 8 heads: 35 us in parts of 512, 42 of 768; one row of 65551, 4 KV heads: 37 us in 384, 41 in 256, 45 in 1024),
+// of at most 1024, which evens out rows of different lengths (32 rows of 300 to 16384, 8 KV heads: 188 us; 213 in 512, 209 in 4096).
 static int paged_chunk(int64_t tiles, int64_t cap) {
-    int64_t chunk = cdiv(cap * tiles, 512);
+    int64_t chunk = cdiv(cap * tiles, 768);
     if (chunk > 1024) chunk = 1024;
-    if (cap <= 512) chunk = cap;
+    if (cap <= 512 || (cap <= 2048 && tiles >= 384)) chunk = cap;
     return (int)(cdiv(chunk, 128) * 128);
 }
 // Joining many splits takes a workgroup of 1024 threads (171 splits of 32 heads: 11 us with 256).
@@ -676,7 +687,7 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.G = (int)(a->H / a->Hkv); p.d = (int)a->d; p.rot = (int)a->rot;
     p.n_pos = a->rot ? (int)a->n_pos : 1; p.ld_q = a->ld_q; p.ld_k = a->ld_k; p.ld_v = a->ld_v; p.scale = (float)(1.0 / sqrt((double)a->d));
     p.chunk = r.chunk; p.nsplit = r.nsplit; p.ctiles = (int)cdiv(p.G, 16); p.stable = a->mode == MM_ATTN_STABLEMAX;
-    const int64_t blocks = a->B * a->Hkv * p.ctiles * p.nsplit;
+    const int64_t blocks = a->B * a->Hkv * p.ctiles * (p.nsplit | 1);
     const int wchunks = a->weights ? (int)cdiv(a->width * a->page, paged_wide_join(r.nsplit) ? 4096 : 1024) : 0, joins = p.nsplit > 1 ? (int)(a->B * a->H) : 0;
     const int64_t blocks2 = joins + a->B * a->Hkv * wchunks;
     MM_CHECK(a->B * a->H < (1LL << 31) && blocks < (1LL << 31) && blocks2 < (1LL << 31), "paged_decode_attn: too many rows and heads for one call");
