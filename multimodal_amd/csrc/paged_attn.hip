@@ -30,7 +30,7 @@ struct PagedP {
     const void* q; const void* kn; const void* vn; void* kpool; void* vpool; void* o; float* w; const int* lengths; const int* positions;
     const float* cos_t; const float* sin_t; PagedMap map;
     float* part; float2* stat; float* sc;       // per (row, head, split): unscaled output [d], (max, sum); scores [row][head][capacity]
-    int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, units, stable; long ld_q, ld_k, ld_v; float scale;
+    int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, heads, units, stable; long ld_q, ld_k, ld_v; float scale;
 };
 
 // Slots of row b that the call attends over (its own token among them), and how they are split: into ceil(cover / chunk) even parts, in whole
@@ -299,14 +299,16 @@ template <typename T, int VE_, int NS_, int NT_, int AL, bool ST> struct Step {
 
 // ------------------------------------------------------------------------------------------------ the walk
 // WPR: waves that share a (row, KV head, split): 4 (merged through LDS), or 1 (four of them side by side in a workgroup).  ST: the cache is
-// read past the last-level cache (non-temporal).
+// read past the last-level cache (non-temporal).  Waves a SIMD: three for heads up to 128, two up to 192, one beyond, where registers
+// would spill -- but for short rows, which wait more than they read (8192 rows and heads of 256, 10 slots: 98 us with one, 68 with two;
+// of 200 to 400 slots 125 and 139).
 template <typename T, int VE, int NS, int NT, int AL, int WPR, bool ST>
-__global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS * sizeof(T) * NT <= 48 ? 2 : 1)) void paged_attn_k(const PagedP p) {
+__global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS * sizeof(T) * NT <= (WPR == 1 ? 64 : 48) ? 2 : 1)) void paged_attn_k(const PagedP p) {
     typedef Step<T, VE, NS, NT, AL, ST> S_t;
     constexpr int SW = 16 * VE, DP = SW * NS, SL = 16 * NT, RD = WPR * SL, J = 4 * NT;    // a wave's step, a round of the waves of a row
-    constexpr int HEADS = WPR == 4 ? 16 : 4, QB = S_t::QT * HEADS * S_t::QS * (int)sizeof(T);   // query heads a tile may have (launch)
-    constexpr int MERGE = WPR == 4 ? 4 * 16 * SW * 4 : 0, TEAMS = 4 / WPR, TT = 64 * WPR;
-    __shared__ __attribute__((aligned(16))) char lds[TEAMS * QB > MERGE ? TEAMS * QB : MERGE];  // q; at the end the waves' outputs
+    constexpr int TEAMS = 4 / WPR, TT = 64 * WPR;
+    extern __shared__ __attribute__((aligned(16))) char lds[];                            // q of the teams; at the end the waves' outputs (paged_lds)
+    const int HEADS = p.heads, QB = S_t::QT * HEADS * S_t::QS * (int)sizeof(T);           // query heads of a tile
     __shared__ __attribute__((aligned(16))) T own_kv[TEAMS][2][DP];
     __shared__ float st_m[4][16], st_l[4][16];
     const int lane = threadIdx.x & 63, wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, g = lane >> 4;
@@ -525,7 +527,7 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
             for (int r = 0; r < 4; r++)
 #pragma unroll
                 for (int e = 0; e < VE; e += 4)
-                    *reinterpret_cast<f32x4_t*>(out + (wave * 16 + li) * SW + (g * 4 + r) * VE + e) =
+                    *reinterpret_cast<f32x4_t*>(out + (wave * HEADS + li) * SW + (g * 4 + r) * VE + e) =
                         f32x4_t{acc[a][e][r] * f, acc[a][e + 1][r] * f, acc[a][e + 2][r] * f, acc[a][e + 3][r] * f};
         lds_barrier();
         for (int i = tid; i < nh * (SW / 4); i += 256) {
@@ -533,7 +535,7 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
             if (a * SW + c >= d) continue;
             f32x4_t v = *reinterpret_cast<f32x4_t*>(out + h * SW + c);
 #pragma unroll
-            for (int w = 1; w < 4; w++) v += *reinterpret_cast<f32x4_t*>(out + (w * 16 + h) * SW + c);
+            for (int w = 1; w < 4; w++) v += *reinterpret_cast<f32x4_t*>(out + (w * HEADS + h) * SW + c);
             const float r[4] = {v[0], v[1], v[2], v[3]};
             const long bh = (long)b * p.H + h0 + h;
             if (single) VecIO<T, 4>::store((T*)p.o + bh * d + a * SW + c, r);
@@ -624,14 +626,14 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
 }
 
 // The most slots of a part, a whole number of rounds of 128.  Not split: up to 512 slots (a second launch costs more than it saves: 24.7 us
-// against 33.5 for 32 rows of 16 heads and 500 slots), and up to 2048 where there are rows and heads for more than one workgroup a CU (512
+// against 33.5 for 32 rows of 16 heads and 500 slots), and up to 2048 where there are rows and heads for a workgroup a CU (512
 // of 1000 to 2000 slots: 75 us, 84 in two parts; 452 heads of 256 and up to 857: 67, 78).  Else parts for about 768 workgroups (16 rows
 // of up to 3000 slots, 8 heads: 35 us in parts of 512, 42 of 768; one row of 65551, 4 KV heads: 37 us in 384, 41 in 256, 45 in 1024),
 // of at most 1024, which evens out rows of different lengths (32 rows of 300 to 16384, 8 KV heads: 188 us; 213 in 512, 209 in 4096).
 static int paged_chunk(int64_t tiles, int64_t cap) {
     int64_t chunk = cdiv(cap * tiles, 768);
     if (chunk > 1024) chunk = 1024;
-    if (cap <= 512 || (cap <= 2048 && tiles >= 384)) chunk = cap;
+    if (cap <= 512 || (cap <= 2048 && tiles >= 256)) chunk = cap;
     return (int)(cdiv(chunk, 128) * 128);
 }
 // Joining many splits takes a workgroup of 1024 threads (171 splits of 32 heads: 11 us with 256).
@@ -656,7 +658,10 @@ extern "C" size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* a) {
 }
 
 template <typename T, int VE, int NS, int NT, int AL> static void paged_launch(const PagedP& p, bool lone, bool past, hipStream_t st) {
-#define MM_PAGED(WPR_, ST_) hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL, WPR_, ST_>), dim3((unsigned)cdiv(p.units, WPR_ == 1 ? 4 : 1)), dim3(256), 0, st, p)
+    typedef Step<T, VE, NS, NT, AL, false> S_t;
+    const size_t qb = (size_t)S_t::QT * p.heads * S_t::QS * sizeof(T), merge = (size_t)4 * p.heads * 16 * VE * sizeof(float);
+    const size_t lds = lone ? 4 * qb : qb > merge ? qb : merge;                // at most 58 KB
+#define MM_PAGED(WPR_, ST_) hipLaunchKernelGGL((paged_attn_k<T, VE, NS, NT, AL, WPR_, ST_>), dim3((unsigned)cdiv(p.units, WPR_ == 1 ? 4 : 1)), dim3(256), lds, st, p)
     if (lone) { if (past) MM_PAGED(1, true); else MM_PAGED(1, false); }
     else { if (past) MM_PAGED(4, true); else MM_PAGED(4, false); }
 #undef MM_PAGED
@@ -686,15 +691,15 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     p.part = r.part ? (float*)ws : nullptr; p.stat = r.stat ? (float2*)(ws + r.part) : nullptr; p.sc = r.sc ? (float*)(ws + r.part + r.stat) : nullptr;
     p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.G = (int)(a->H / a->Hkv); p.d = (int)a->d; p.rot = (int)a->rot;
     p.n_pos = a->rot ? (int)a->n_pos : 1; p.ld_q = a->ld_q; p.ld_k = a->ld_k; p.ld_v = a->ld_v; p.scale = (float)(1.0 / sqrt((double)a->d));
-    p.chunk = r.chunk; p.nsplit = r.nsplit; p.ctiles = (int)cdiv(p.G, 16); p.stable = a->mode == MM_ATTN_STABLEMAX;
+    p.chunk = r.chunk; p.nsplit = r.nsplit; p.ctiles = (int)cdiv(p.G, 16); p.heads = p.G < 16 ? p.G : 16; p.stable = a->mode == MM_ATTN_STABLEMAX;
     const int64_t blocks = a->B * a->Hkv * p.ctiles * (p.nsplit | 1);
     const int wchunks = a->weights ? (int)cdiv(a->width * a->page, paged_wide_join(r.nsplit) ? 4096 : 1024) : 0, joins = p.nsplit > 1 ? (int)(a->B * a->H) : 0;
     const int64_t blocks2 = joins + a->B * a->Hkv * wchunks;
     MM_CHECK(a->B * a->H < (1LL << 31) && blocks < (1LL << 31) && blocks2 < (1LL << 31), "paged_decode_attn: too many rows and heads for one call");
     p.units = (int)blocks;
     // Many short rows: a wave each (1024 rows of 160 to 238 slots, 8 heads: 164 us, four waves a row 173; 256 rows of 900, 8 KV heads: 150 and 140).
-    // A tile of more than four heads would not find its q in that variant's LDS.
-    const bool lone = p.G <= 4 && r.nsplit == 1 && a->width * a->page <= 512 && blocks >= 2048;
+    // Four times q in LDS: not for more than four query heads a KV head unless the head is small.
+    const bool lone = (p.G <= 4 || a->d <= 64) && r.nsplit == 1 && a->width * a->page <= 512 && blocks >= 2048;
     // A cache that the last-level cache (256 MB) cannot hold until the next call is read past it: 154 us for 164 at 849 MB; at 69 MB it
     // would be 39 for 26.
     const bool past = a->B * a->Hkv * a->width * a->page * a->d * (a->dtype == MM_BF16 ? 4 : 8) > (256LL << 20);

@@ -206,40 +206,61 @@ template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& 
             }
     }
 }
-// the newest slots, down by n - budget: one chain (residue class) and piece a thread
-template <typename U> __device__ __forceinline__ void evict_shift(const EvictP& p, int b, int h, int t, int step) {
+// The newest slots, down by n - budget, by `blocks` workgroups of NT threads: a chain (residue class) and piece a thread where there are enough
+// of them.  Few chains are long ones (one token over the budget: one chain of all the newest slots): then one workgroup moves tile
+// after tile instead, all loads of a tile before its stores, which only overwrite what has been loaded (96 heads of 964 newest slots, some
+// rows one slot over: 550 us in chains).
+template <typename U, int NT> __device__ __forceinline__ void evict_shift(const EvictP& p, int b, int h, int block, int blocks) {
     const int n = p.head((long)b * p.map.Hkv + h)[0];
-    if (n <= p.budget) return;
-    const int by = n - p.budget, first = n - p.recent;
-    const unsigned total = (unsigned)min(by, p.recent) * (unsigned)p.units;
+    if (n <= p.budget || !p.recent) return;
+    const int by = n - p.budget, first = n - p.recent, tid = threadIdx.x;
+    const unsigned total = (unsigned)min(by, p.recent) * (unsigned)p.units, all = (unsigned)p.recent * (unsigned)p.units;
     U* K = (U*)p.kpool; U* V = (U*)p.vpool;
     constexpr int N = 4;
-    for (unsigned i = t; i < total; i += (unsigned)step) {
-        const unsigned c = i / (unsigned)p.units;
-        const int piece = (int)(i - c * (unsigned)p.units);
-        for (long j0 = c; j0 < p.recent; j0 += (long)N * by) {
+    auto take = [&](long j, int piece, long& d, U& k, U& v, float& w) {
+        const long s = p.map.row(b, h, first + (int)j);
+        d = -1;
+        if (s >= 0) {
+            d = p.map.row(b, h, first + (int)j - by);
+            k = K[s * p.units + piece]; v = V[s * p.units + piece];
+            if (piece == 0) w = p.w[s];
+        }
+    };
+    auto put = [&](int piece, long d, const U& k, const U& v, float w) {
+        if (d < 0) return;
+        K[d * p.units + piece] = k; V[d * p.units + piece] = v;
+        if (piece == 0) p.w[d] = w;
+    };
+    if (total >= all || total >= NT / 2) {
+        for (unsigned i = (unsigned)(block * NT + tid); i < total; i += (unsigned)(blocks * NT)) {
+            const unsigned c = i / (unsigned)p.units;
+            const int piece = (int)(i - c * (unsigned)p.units);
+            for (long j0 = c; j0 < p.recent; j0 += (long)N * by) {
+                U k[N], v[N];
+                float w[N];
+                long d[N];
+#pragma unroll
+                for (int e = 0; e < N; e++) { const long j = j0 + (long)e * by; d[e] = -1; if (j < p.recent) take(j, piece, d[e], k[e], v[e], w[e]); }
+#pragma unroll
+                for (int e = 0; e < N; e++) put(piece, d[e], k[e], v[e], w[e]);
+            }
+        }
+    } else if (block == 0) {
+        for (unsigned i0 = 0; i0 < all; i0 += NT * N) {
             U k[N], v[N];
             float w[N];
             long d[N];
+            int piece[N];
 #pragma unroll
             for (int e = 0; e < N; e++) {
-                const long j = j0 + (long)e * by;
+                const unsigned i = i0 + (unsigned)(e * NT + tid), j = i / (unsigned)p.units;
+                piece[e] = (int)(i - j * (unsigned)p.units);
                 d[e] = -1;
-                if (j < p.recent) {
-                    const long s = p.map.row(b, h, first + (int)j);
-                    if (s >= 0) {
-                        d[e] = p.map.row(b, h, first + (int)j - by);
-                        k[e] = K[s * p.units + piece]; v[e] = V[s * p.units + piece];
-                        if (piece == 0) w[e] = p.w[s];
-                    }
-                }
+                if (i < all) take(j, piece[e], d[e], k[e], v[e], w[e]);
             }
+            __syncthreads();
 #pragma unroll
-            for (int e = 0; e < N; e++)
-                if (d[e] >= 0) {
-                    K[d[e] * p.units + piece] = k[e]; V[d[e] * p.units + piece] = v[e];
-                    if (piece == 0) p.w[d[e]] = w[e];
-                }
+            for (int e = 0; e < N; e++) put(piece[e], d[e], k[e], v[e], w[e]);
         }
     }
 }
@@ -258,7 +279,7 @@ template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW *
         __syncthreads();
         evict_moves<U>(p, b, h, threadIdx.x, NW * 64);
         __syncthreads();                                                       // targets of the shift were sources of the moves
-        evict_shift<U>(p, b, h, threadIdx.x, NW * 64);
+        evict_shift<U, NW * 64>(p, b, h, 0, 1);
     }
 }
 // The last launch writes the new lengths: only the selection reads the old ones.
@@ -269,8 +290,8 @@ template <typename U, bool LAST> __global__ __launch_bounds__(256) void evict_mo
     evict_moves<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
     if constexpr (LAST) evict_length(p, blockIdx.x);
 }
-template <typename U> __global__ __launch_bounds__(256) void evict_shift_k(const EvictP p) {
-    evict_shift<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
+template <typename U> __global__ __launch_bounds__(1024) void evict_shift_k(const EvictP p) {
+    evict_shift<U, 1024>(p, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z);
     evict_length(p, blockIdx.x);
 }
 __global__ __launch_bounds__(64) void evict_lengths_k(const EvictP p) { evict_length(p, blockIdx.x); }
@@ -294,8 +315,8 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
                                      else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
     if (cap <= 1024) MM_SELECT(4, 4);
     else if (cap <= 8192) MM_SELECT(8, 16);                               // eight waves: 26 us for 384 heads of 8192 slots, 16 waves 37, four 33
-    else if (cap <= 32768) MM_SELECT(8, 64);
-    else if (cap <= 65536) MM_SELECT(8, 128);
+    else if (cap <= 32768) MM_SELECT(16, 32);
+    else if (cap <= 65536) MM_SELECT(16, 64);
     else MM_SELECT(16, 0);
 #undef MM_SELECT
     auto split = [&](int64_t items) {                                          // workgroups per (row, KV head): four pieces a thread, 4096 workgroups in all
@@ -307,7 +328,10 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
         if (p.recent) hipLaunchKernelGGL((evict_moves_k<U, false>), g, dim3(256), 0, st, p);
         else hipLaunchKernelGGL((evict_moves_k<U, true>), g, dim3(256), 0, st, p);
     }
-    if (!all && p.recent) hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, split((int64_t)p.recent * p.units)), dim3(256), 0, st, p);
+    if (!all && p.recent) {
+        const int64_t w = cdiv((int64_t)p.recent * p.units, 4096), most = cdiv(1024, heads);
+        hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, (unsigned)(w < 1 ? 1 : w < most ? w : most)), dim3(1024), 0, st, p);
+    }
     if (all) hipLaunchKernelGGL(evict_lengths_k, dim3(grid.x), dim3(64), 0, st, p);
 }
 
