@@ -261,11 +261,11 @@ typedef struct {
     int64_t B, H, Hkv, d, rot, page, n_pages, width, ld_table, ld_q, ld_k, ld_v, n_pos;
     int mode;                   /* MM_ATTN_SOFTMAX | MM_ATTN_STABLEMAX */
     int dtype;
-    void* workspace; size_t workspace_bytes;   /* mm_paged_decode_attn_workspace(args): private to the call until it has run */
+    void* workspace; size_t workspace_bytes;   /* mm_paged_decode_attn_workspace(args), 16-byte aligned: private to the call until it has run */
 } mm_paged_attn_args;
 /* One token of every row: q and k_new are rotated (half layout, first rot dims) at the row's position, k_new (rotated, rounded to
  * the cache's type) and v_new are stored at slot lengths[b], and q attends over slots 0 .. lengths[b] (over 0 .. lengths[b] - 1
- * without k_new).  lengths is not changed.  A row without a slot gets o = 0.  Scores, softmax statistics, sums and weights are
+ * without k_new).  lengths is not changed.  A row without a slot, and one whose scores are all -inf, gets o = 0.  Scores, softmax statistics, sums and weights are
  * float32; results do not depend on what else runs (no atomics). */
 size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* args);
 int mm_paged_decode_attn(const mm_paged_attn_args* args, void* stream);

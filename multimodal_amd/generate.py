@@ -389,7 +389,7 @@ def speculative_generate(model, draft, nmr_tokens: Optional[torch.Tensor], ir_da
             out.scatter_(1, at, torch.where(done[:, None], out.gather(1, at), torch.where(keep, new, torch.full_like(new, pad_id))))
             cur = new.gather(1, accepted[:, None])[:, 0]
             more = torch.where(done, torch.zeros_like(accepted), accepted + 1)
-            said += more
+            said = (said + more).clamp(max=steps)      # what a row says past the end is cut off with it
             held = [n + more.to(torch.int32) for n in held]
             done = done | (end < T) | (said >= steps)
             if bool(done.all()):

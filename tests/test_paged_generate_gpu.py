@@ -122,6 +122,24 @@ def test_drafted_greedy_ids_are_the_greedy_ids(same, n_draft):
         assert all(x == n_draft for x in counts[0])
 
 
+def test_rows_that_end_at_different_times():
+    """Many rows, long drafts, few tokens: rows reach the end several passes apart, some in the middle of an accepted run."""
+    from multimodal_amd.generate import speculative_generate
+    m, d = _model(11), _model(12, E=64, L=1)
+    with torch.no_grad():                                                      # drafts that are often, not always, right
+        d.decoder.out.weight.zero_(); d.decoder.out.bias.copy_(m.decoder.out.bias)
+        m.decoder.out.weight.mul_(0.1); m.decoder.out.bias.mul_(30)
+        d.decoder.out.bias.copy_(m.decoder.out.bias)
+    nmr, ir = _inputs(64)
+    for max_len in (1, 2, 7, 15):
+        got = speculative_generate(m, d, nmr, ir, max_len=max_len, n_draft=8, temperature=1.0, generator=torch.Generator(device=DEV).manual_seed(3))
+        torch.cuda.synchronize()
+        assert got.shape[1] <= max_len + 1 and ((got >= 0) & (got < 591)).all()
+        want = m.generate(nmr, ir, max_len=max_len, early_stop=False)
+        again = speculative_generate(m, d, nmr, ir, max_len=max_len, n_draft=8, temperature=0, eos_id=-7)
+        assert torch.equal(again, want)
+
+
 def test_drafted_samples_are_repeatable_and_valid():
     from multimodal_amd.generate import speculative_generate
     m, d = _model(9), _model(10, E=64, L=1)

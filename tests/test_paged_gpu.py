@@ -406,6 +406,40 @@ def test_shared_prompt_pages_and_repeated_rows():
         assert torch.equal(oe[b:b + 1], ops.paged_decode_attn(q[b:b + 1], None, None, c.k, c.v, c.table[:1], n[:1], 2, 0, None, None, False))
 
 
+@pytest.mark.parametrize("dtype,d,rot", [(torch.bfloat16, 64, 64), (torch.bfloat16, 100, 50), (torch.float32, 64, 32), (torch.float32, 36, 6)])
+def test_rows_at_odd_addresses(dtype, d, rot):
+    """q, k and v as views whose rows start at any multiple of a value's size: the step and the run."""
+    from multimodal_amd import ops
+    lens = [40, 0, 17]
+    Hkv, G = 2, 3
+    c, q, k, v = _filled(16, dtype, 3, Hkv, G, d, 16, lens, weights=True)
+    g = torch.Generator().manual_seed(17)
+    odd = lambda *s: _randn(g, *s[:-1], s[-1] + 7, dtype=dtype).to(DEV)[..., 3: 3 + s[-1]]
+    q, k, v = odd(3, Hkv * G * d), odd(3, Hkv * d), odd(3, Hkv * d)
+    assert q.data_ptr() % 4 == (2 if dtype == torch.bfloat16 else 0)
+    before = (c.k.clone(), c.v.clone(), c.w.clone())
+    tabs = _tables(rot, 50)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = ops.paged_decode_attn(q, k, v, c.k, c.v, c.table, n, Hkv * G, rot, *tabs, False, weights=c.w)
+    _check_step(c, before, q, k, v, lens, Hkv * G, rot, tabs, False, None, o)
+    kk, vv = odd(3, 4, Hkv * d), odd(3, 4, Hkv * d)
+    a, b = Cache(19, dtype, 3, Hkv, d, 16, [60] * 3), Cache(19, dtype, 3, Hkv, d, 16, [60] * 3)
+    ops.paged_cache_fill(kk, vv, a.k, a.v, a.table, rot, *tabs, start=n)
+    ops.paged_cache_fill(kk.contiguous(), vv.contiguous(), b.k, b.v, b.table, rot, *tabs, start=n)
+    assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8)) and torch.equal(a.v.view(torch.uint8), b.v.view(torch.uint8))
+
+
+def test_all_scores_minus_infinity():
+    """Every key infinitely far away: a row without weight gets zeros."""
+    from multimodal_amd import ops
+    for dtype in (torch.bfloat16, torch.float32):
+        c, q, k, v = _filled(20, dtype, 1, 1, 1, 64, 16, [40])
+        q = q.clone().fill_(1.0)
+        c.k[c.table[0].long()] = -math.inf
+        o = ops.paged_decode_attn(q, None, None, c.k, c.v, c.table, torch.tensor([40], dtype=torch.int32, device=DEV), 1, 0, None, None, False)
+        assert (o == 0).all()
+
+
 def test_agrees_with_the_dense_cache_step():
     """The same step through ops.decode_attn's dense cache: float32, both normalisations."""
     from multimodal_amd import ops
