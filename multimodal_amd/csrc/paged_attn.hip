@@ -33,7 +33,7 @@ typedef f32x4_t __attribute__((aligned(4))) f4_4_t;
 struct PagedP {
     const void* q; const void* kn; const void* vn; void* kpool; void* vpool; void* o; float* w; const int* lengths; const int* positions;
     const float* cos_t; const float* sin_t; PagedMap map;
-    float* part; float2* stat; float* sc;       // per (row, head, split): unscaled output [d], (max, sum); scores [row][head][capacity]
+    float* part; float2* stat; float* sc; float* sc_own;   // per (row, head, split): unscaled output [d], (max, sum); scores [row][head][capacity], [row][head]
     int B, H, Hkv, G, d, rot, n_pos, chunk, nsplit, ctiles, heads, units, stable; long ld_q, ld_k, ld_v; float scale;
 };
 
@@ -422,22 +422,21 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
         for (int e = 0; e < VE; e++) acc[s][e] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     const float sc = p.stable ? p.scale : p.scale * 1.44269504088896340736f;            // softmax in base 2
-    float* srow = p.sc ? p.sc + ((long)b * p.H + h0 + li) * cap : nullptr;
+    float* srow = p.sc + ((long)b * p.H + h0 + li) * cap;
     // from the scores of a step to its probabilities (relative to the running maximum), which rescale what was gathered before
     auto weigh = [&](const f32x4_t (&s)[NT], unsigned okb, float (&pr)[J], int slot) {
         float x[J];
 #pragma unroll
         for (int j = 0; j < J; j++) x[j] = s[j >> 2][j & 3] * sc;
-        if (srow && li < nh) {
+        // the scores, for the weights: four slots at once, those past the end among them (nothing reads them).  The new token's score goes to a place
+        // of its own, as its slot is among another wave's four.
+        if (p.sc && li < nh) {
+            if (slot >= 0) {
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
-                const unsigned bits = okb >> (t * 4) & 15;
-                if (slot >= 0 && bits == 15) *reinterpret_cast<f32x4_t*>(srow + slot + t * 16 + g * 4) = f32x4_t{x[t * 4], x[t * 4 + 1], x[t * 4 + 2], x[t * 4 + 3]};
-                else if (slot >= 0) {                                                   // the last slots: the new token's score is another wave's
-#pragma unroll
-                    for (int i = 0; i < 4; i++) if (bits >> i & 1) srow[slot + t * 16 + g * 4 + i] = x[t * 4 + i];
-                } else if (bits) srow[len] = x[0];
-            }
+                for (int t = 0; t < NT; t++)
+                    if (slot + t * 16 + g * 4 < hi)
+                        *reinterpret_cast<f32x4_t*>(srow + slot + t * 16 + g * 4) = f32x4_t{x[t * 4], x[t * 4 + 1], x[t * 4 + 2], x[t * 4 + 3]};
+            } else if (g == 0) p.sc_own[b * p.H + h0 + li] = x[0];
         }
         if (p.stable) {
 #pragma unroll
@@ -599,6 +598,7 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
     const int part = paged_part(p, n), ns = (n + part - 1) / part, cap = p.map.capacity();
     const int slot = s0 + tid * 4;
     const long row = slot < n ? p.map.row(b, hk, slot) : -1;                            // four slots of one page (page >= 4)
+    const int fresh = p.kn ? len - slot : -1;                                           // which of the four is the new token
     f32x4_t old = {0.f, 0.f, 0.f, 0.f}, add = old;
     if (row >= 0) old = *reinterpret_cast<const f32x4_t*>(p.w + row);
     for (int g0 = 0; g0 < p.G; g0 += 64) {
@@ -614,18 +614,19 @@ template <typename T, int NTH> __global__ __launch_bounds__(NTH) void paged_join
         if (row >= 0)
 #pragma unroll 4
             for (int h = 0; h < ng; h++) {
-                const f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.sc + (bh + h) * cap + slot);
+                f32x4_t x = *reinterpret_cast<const f32x4_t*>(p.sc + (bh + h) * cap + slot);
+                if (fresh >= 0 && fresh < 4) x[fresh] = p.sc_own[bh + h];
 #pragma unroll
                 for (int i = 0; i < 4; i++) add[i] += (p.stable ? stable_s(x[i]) : __builtin_amdgcn_exp2f(x[i] - hb[h])) * hi[h];
             }
     }
     if (row < 0) return;
-    if (slot + 4 <= n && !(p.kn && slot + 4 > len)) {
+    if (slot + 4 <= n && !(fresh >= 0 && fresh < 4)) {
         *reinterpret_cast<f32x4_t*>(p.w + row) = old + add;
     } else {
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            if (slot + i < n) p.w[row + i] = p.kn && slot + i == len ? add[i] : old[i] + add[i];
+            if (slot + i < n) p.w[row + i] = i == fresh ? add[i] : old[i] + add[i];
     }
 }
 
@@ -642,7 +643,7 @@ static int paged_chunk(int64_t tiles, int64_t cap) {
 }
 // Joining many splits takes a workgroup of 1024 threads (171 splits of 32 heads: 11 us with 256).
 static bool paged_wide_join(int nsplit) { return nsplit > 32; }
-struct PagedPlan { int chunk, nsplit; size_t part, stat, sc; };
+struct PagedPlan { int chunk, nsplit; size_t part, stat, sc, own; };
 static PagedPlan paged_plan(const mm_paged_attn_args* a) {
     const int64_t cap = a->width * a->page, tiles = a->B * a->Hkv * cdiv(a->H / a->Hkv, 16);
     PagedPlan r;
@@ -652,13 +653,14 @@ static PagedPlan paged_plan(const mm_paged_attn_args* a) {
     r.stat = r.nsplit > 1 || a->weights ? (size_t)(a->B * a->H) * r.nsplit * sizeof(float2) : 0;
     r.stat = (r.stat + 15) / 16 * 16;
     r.sc = a->weights ? (size_t)(a->B * a->H) * cap * sizeof(float) : 0;
+    r.own = a->weights ? (size_t)(a->B * a->H) * sizeof(float) : 0;
     return r;
 }
 
 extern "C" size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* a) {
     if (!a || a->B <= 0 || a->H <= 0 || a->Hkv <= 0 || a->H < a->Hkv || a->d <= 0 || a->width <= 0 || a->page <= 0) return 0;
     const PagedPlan r = paged_plan(a);
-    return r.part + r.stat + r.sc;
+    return r.part + r.stat + r.sc + r.own;
 }
 
 template <typename T, int VE, int NS, int NT, int AL> static void paged_launch(const PagedP& p, bool lone, bool past, hipStream_t st) {
@@ -684,7 +686,7 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     MM_CHECK(a->mode == MM_ATTN_SOFTMAX || a->mode == MM_ATTN_STABLEMAX, "paged_decode_attn: bad mode %d", a->mode);
     MM_CHECK((((uintptr_t)a->o | (uintptr_t)a->weights) % 16) == 0, "paged_decode_attn: o and weights must be 16-byte aligned");
     const PagedPlan r = paged_plan(a);
-    const size_t need = r.part + r.stat + r.sc;
+    const size_t need = r.part + r.stat + r.sc + r.own;
     MM_CHECK(need == 0 || (a->workspace && a->workspace_bytes >= need && ((uintptr_t)a->workspace % 16) == 0), "paged_decode_attn: workspace too small or not 16-byte aligned");
     hipStream_t st = (hipStream_t)stream;
     PagedP p{};
@@ -693,6 +695,7 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     p.map = {a->page_table, (long)a->ld_table, (int)a->width, paged_shift(a->page), (int)a->n_pages, (int)a->Hkv};
     char* ws = (char*)a->workspace;
     p.part = r.part ? (float*)ws : nullptr; p.stat = r.stat ? (float2*)(ws + r.part) : nullptr; p.sc = r.sc ? (float*)(ws + r.part + r.stat) : nullptr;
+    p.sc_own = (float*)(ws + r.part + r.stat + r.sc);
     p.B = (int)a->B; p.H = (int)a->H; p.Hkv = (int)a->Hkv; p.G = (int)(a->H / a->Hkv); p.d = (int)a->d; p.rot = (int)a->rot;
     p.n_pos = a->rot ? (int)a->n_pos : 1; p.ld_q = a->ld_q; p.ld_k = a->ld_k; p.ld_v = a->ld_v; p.scale = (float)(1.0 / sqrt((double)a->d));
     p.chunk = r.chunk; p.nsplit = r.nsplit; p.ctiles = (int)cdiv(p.G, 16); p.heads = p.G < 16 ? p.G : 16; p.stable = a->mode == MM_ATTN_STABLEMAX;
