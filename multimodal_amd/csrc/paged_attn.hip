@@ -656,7 +656,7 @@ static PagedPlan paged_plan(const mm_paged_attn_args* a) {
     r.nsplit = (int)cdiv(cap, r.chunk);
     r.part = r.nsplit > 1 ? (size_t)(a->B * a->H) * r.nsplit * a->d * sizeof(float) : 0;
     r.stat = r.nsplit > 1 || a->weights ? (size_t)(a->B * a->H) * r.nsplit * sizeof(float2) : 0;
-    r.stat = (r.stat + 15) / 16 * 16;
+    r.stat = (r.stat + 255) / 256 * 256;                                                // whole cache lines of scores
     r.sc = a->weights ? (size_t)(a->B * a->H) * cap * sizeof(float) : 0;
     r.own = a->weights ? (size_t)(a->B * a->H) * sizeof(float) : 0;
     return r;

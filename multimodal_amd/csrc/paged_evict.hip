@@ -329,7 +329,7 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
         else hipLaunchKernelGGL((evict_moves_k<U, true>), g, dim3(256), 0, st, p);
     }
     if (!all && p.recent) {
-        const int64_t w = cdiv((int64_t)p.recent * p.units, 4096), most = cdiv(1024, heads);
+        const int64_t w = cdiv((int64_t)p.recent * p.units, 1024), most = cdiv(2048, heads);   // a piece a thread
         hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, (unsigned)(w < 1 ? 1 : w < most ? w : most)), dim3(1024), 0, st, p);
     }
     if (all) hipLaunchKernelGGL(evict_lengths_k, dim3(grid.x), dim3(64), 0, st, p);
