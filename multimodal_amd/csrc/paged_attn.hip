@@ -27,7 +27,8 @@
 typedef __attribute__((ext_vector_type(4))) unsigned u4_t;
 typedef __attribute__((ext_vector_type(2))) unsigned u2_t;
 typedef u4_t __attribute__((aligned(8))) u4_8_t;
-typedef u4_t __attribute__((aligned(2))) u4_2_t;                    // rows of q and the new key need no alignment beyond a value's
+typedef u4_t __attribute__((aligned(2))) u4_2_t;                    // rows that are read once need no alignment beyond a value's
+typedef u2_t __attribute__((aligned(2))) u2_2_t;
 typedef f32x4_t __attribute__((aligned(4))) f4_4_t;
 
 struct PagedP {
@@ -53,48 +54,56 @@ __device__ __forceinline__ int paged_pos(const int* positions, const int* length
     const int pos = positions ? positions[b] : (append ? n : n - 1);
     return min(max(pos, 0), n_pos - 1);
 }
-// values c .. c + 7 (bf16) or c + 3 (f32) of a row of d, 0 past its end
-__device__ __forceinline__ void raw_piece(const bf16* x, int c, int d, float (&v)[8]) {
-    if (c + 8 <= d) {
-        const u4_t w = *reinterpret_cast<const u4_2_t*>(x + c);
+// VE consecutive values from any address a value may have
+template <int VE> __device__ __forceinline__ void load_any(const bf16* x, float (&v)[VE]) {
+    unsigned w[VE / 2];
+    if constexpr (VE == 8) {
+        const u4_t t = *reinterpret_cast<const u4_2_t*>(x);
+        w[0] = t[0]; w[1] = t[1]; w[2] = t[2]; w[3] = t[3];
+    } else {
+        const u2_t t = *reinterpret_cast<const u2_2_t*>(x);
+        w[0] = t[0]; w[1] = t[1];
+    }
 #pragma unroll
-        for (int i = 0; i < 4; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-    } else
-#pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = c + i < d ? to_f(x[c + i]) : 0.f;
+    for (int i = 0; i < VE / 2; i++) { v[2 * i] = __uint_as_float(w[i] << 16); v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 }
-__device__ __forceinline__ void raw_piece(const float* x, int c, int d, float (&v)[4]) {
-    const f32x4_t w = c < d ? *reinterpret_cast<const f4_4_t*>(x + c) : f32x4_t{0.f, 0.f, 0.f, 0.f};    // d % 4 == 0
+template <int VE> __device__ __forceinline__ void load_any(const float* x, float (&v)[VE]) {
 #pragma unroll
-    for (int i = 0; i < 4; i++) v[i] = w[i];
+    for (int e = 0; e < VE; e += 4) {
+        const f32x4_t t = *reinterpret_cast<const f4_4_t*>(x + e);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[e + i] = t[i];
+    }
 }
-// the same, rotated (half layout over the first rot values) at the table row cs / sn
-template <typename T, int PE> __device__ __forceinline__ void piece(const T* x, int c, int d, int rot, const float* cs, const float* sn, float (&v)[PE]) {
-    raw_piece(x, c, d, v);
+// the same of a row of d, 0 past its end (d % 4 == 0)
+template <typename T, int VE> __device__ __forceinline__ void raw_piece(const T* x, int c, int d, float (&v)[VE]) {
+    if (c + VE <= d) load_any(x + c, v);
+    else
+#pragma unroll
+        for (int e = 0; e < VE; e++) v[e] = c + e < d ? to_f(x[c + e]) : 0.f;
+}
+// values c .. c + VE - 1 of a row, v, rotated (half layout over the first rot values) at the table row cs / sn
+template <typename T, int VE> __device__ __forceinline__ void turn(const T* x, int c, int rot, const float* cs, const float* sn, float (&v)[VE]) {
     if (c >= rot) return;
     const int half = rot >> 1;
-    if (half % PE == 0) {
-        const bool low = c < half;
+    const bool low = c < half;
+    if (low ? c + VE <= half : c + VE <= rot) {                                // within one half: partners and angles are consecutive too
         const int i = low ? c : c - half;
-        float o[PE], cv[PE], sv[PE];
-        raw_piece(x, low ? c + half : i, d, o);
+        float o[VE], cv[VE], sv[VE];
+        load_any(x + (low ? c + half : i), o);
+        load_any(cs + i, cv);
+        load_any(sn + i, sv);
 #pragma unroll
-        for (int e = 0; e < PE; e += 4) {
-            const f32x4_t a = *reinterpret_cast<const f4_4_t*>(cs + i + e), b = *reinterpret_cast<const f4_4_t*>(sn + i + e);
-#pragma unroll
-            for (int k = 0; k < 4; k++) { cv[e + k] = a[k]; sv[e + k] = b[k]; }
-        }
-#pragma unroll
-        for (int e = 0; e < PE; e++) v[e] = low ? fmaf(v[e], cv[e], -(o[e] * sv[e])) : fmaf(v[e], cv[e], o[e] * sv[e]);
+        for (int e = 0; e < VE; e++) v[e] = low ? fmaf(v[e], cv[e], -(o[e] * sv[e])) : fmaf(v[e], cv[e], o[e] * sv[e]);
         return;
     }
 #pragma unroll
-    for (int e = 0; e < PE; e++)
+    for (int e = 0; e < VE; e++)
         if (c + e < rot) {
-            const bool low = c + e < half;
-            const int i = low ? c + e : c + e - half;
-            const float o = to_f(x[low ? c + e + half : i]);
-            v[e] = low ? fmaf(v[e], cs[i], -(o * sn[i])) : fmaf(v[e], cs[i], o * sn[i]);
+            const bool first = c + e < half;
+            const int i = first ? c + e : c + e - half;
+            const float o = to_f(x[first ? c + e + half : i]);
+            v[e] = first ? fmaf(v[e], cs[i], -(o * sn[i])) : fmaf(v[e], cs[i], o * sn[i]);
         }
 }
 // stablemax's s(x); the reciprocal is within one unit in the last place
@@ -392,14 +401,18 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
     for (int i = tid; i < nh * PIECES; i += TT) {
         const int h = i / PIECES, c = i % PIECES * PE;
         float x[PE];
-        piece((const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d, c, d, p.rot, cs, sn, x);
+        const T* row = (const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d;
+        raw_piece(row, c, d, x);
+        turn(row, c, p.rot, cs, sn, x);
         S_t::put_q(qlds, HEADS, h, c, x);
     }
     if (mine)
         for (int i = tid; i < PIECES; i += TT) {
             const int c = i * PE;
             float x[PE], y[PE];
-            piece((const T*)p.kn + (long)b * p.ld_k + (long)hk * d, c, d, p.rot, cs, sn, x);
+            const T* row = (const T*)p.kn + (long)b * p.ld_k + (long)hk * d;
+            raw_piece(row, c, d, x);
+            turn(row, c, p.rot, cs, sn, x);
             raw_piece((const T*)p.vn + (long)b * p.ld_v + (long)hk * d, c, d, y);
             VecIO<T, PE>::store(own_k + c, x); VecIO<T, PE>::store(own_v + c, y);       // the key rounded to the cache's type, as it is stored
             if (own_row >= 0 && ct == 0) {
@@ -747,15 +760,15 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
 }
 
 // ------------------------------------------------------------------------------------------------ runs of keys and values
-// A copy: keys and values are read once and written once, which HBM bounds.  A lane moves VE consecutive values of one head of one token;
-// for a rotated key it also reads the partner values (the other half: in the same row, so from the cache that has just fetched it),
-// which spares an exchange between lanes.  VE = 8 (bf16) or 4 (f32) where head_dim and the strides are multiples of it and the rows are
-// aligned, else 1; PV: the halves are multiples of VE too, so that partners are loaded as wide.
+// A copy: keys and values are read once and written once, which HBM bounds: 1125 MB (1024 rows of 100 to 159 tokens, 8 heads of 128, bf16) in
+// 213 us = 5.3 TB/s.  A lane moves VE consecutive values of one head of one token (16 bytes; 8 where a bf16 row is no multiple of 16);
+// for a rotated key it also reads the partner values (the other half: in the same row, so from the cache that has just fetched it), which
+// spares an exchange between lanes.  One piece a lane: with two or four in flight the large case took 230 and 271 us.
 struct FillP {
     const void* k; const void* v; void* kpool; void* vpool; float* w; const int* start; const int* counts; const int* positions;
     const float* cos_t; const float* sin_t; PagedMap map; int S, Hkv, d, rot, n_pos; long ld_k, bs_k, ld_v, bs_v;
 };
-template <typename T, int VE, bool PV> __global__ __launch_bounds__(256) void paged_fill_k(const FillP p) {
+template <typename T, int VE> __global__ __launch_bounds__(256) void paged_fill_k(const FillP p) {
     const int b = blockIdx.y;
     const unsigned pieces = (unsigned)p.d / VE, per = pieces * (unsigned)p.Hkv;
     const unsigned idx = blockIdx.x * 256u + threadIdx.x;                // over [S][Hkv][d / VE]; fits (checked by the launch)
@@ -767,32 +780,12 @@ template <typename T, int VE, bool PV> __global__ __launch_bounds__(256) void pa
     const T* k = (const T*)p.k + (long)b * p.bs_k + (long)s * p.ld_k + (long)h * p.d;
     const T* v = (const T*)p.v + (long)b * p.bs_v + (long)s * p.ld_v + (long)h * p.d;
     float x[VE], y[VE];
-    VecIO<T, VE>::load(k + c, x);
-    VecIO<T, VE>::load(v + c, y);
-    const int half = p.rot >> 1;
+    load_any(k + c, x);
+    load_any(v + c, y);
     if (c < p.rot) {
         const long pos = p.positions ? (long)p.positions[b] + s : (long)st + s;
-        const long t = min(max(pos, 0L), (long)p.n_pos - 1) * half;
-        if constexpr (PV) {
-            const bool low = c < half;
-            const int i = low ? c : c - half;
-            float o[VE];
-            VecIO<T, VE>::load(k + (low ? c + half : i), o);
-#pragma unroll
-            for (int e = 0; e < VE; e++) {
-                const float cs = p.cos_t[t + i + e], sn = p.sin_t[t + i + e];
-                x[e] = low ? fmaf(x[e], cs, -(o[e] * sn)) : fmaf(x[e], cs, o[e] * sn);
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < VE; e++)
-                if (c + e < p.rot) {
-                    const bool low = c + e < half;
-                    const int i = low ? c + e : c + e - half;
-                    const float o = to_f(k[low ? c + e + half : i]), cs = p.cos_t[t + i], sn = p.sin_t[t + i];
-                    x[e] = low ? fmaf(x[e], cs, -(o * sn)) : fmaf(x[e], cs, o * sn);
-                }
-        }
+        const long t = min(max(pos, 0L), (long)p.n_pos - 1) * (p.rot >> 1);
+        turn(k, c, p.rot, p.cos_t + t, p.sin_t + t, x);
     }
     const long row = p.map.row(b, h, st + s);
     if (row < 0) return;
@@ -816,20 +809,14 @@ extern "C" int mm_paged_cache_fill(const mm_paged_fill_args* a, void* stream) {
     p.cos_t = a->cos_t; p.sin_t = a->sin_t; p.map = {a->page_table, (long)a->ld_table, (int)a->width, paged_shift(a->page), (int)a->n_pages, (int)a->Hkv};
     p.S = (int)a->S; p.Hkv = (int)a->Hkv; p.d = (int)a->d; p.rot = (int)a->rot; p.n_pos = a->rot ? (int)a->n_pos : 1;
     p.ld_k = a->ld_k; p.bs_k = a->bs_k; p.ld_v = a->ld_v; p.bs_v = a->bs_v;
-    const int VE = a->dtype == MM_BF16 ? 8 : 4;
-    const int64_t all = a->d | a->ld_k | a->bs_k | a->ld_v | a->bs_v;
-    const bool wide = all % VE == 0 && (((uintptr_t)a->k | (uintptr_t)a->v) % 16) == 0, pv = a->rot / 2 % VE == 0;
-    const int64_t items = a->S * a->Hkv * (a->d / (wide ? VE : 1));
+    const int VE = a->dtype == MM_BF16 && a->d % 8 == 0 ? 8 : 4;
+    const int64_t items = a->S * a->Hkv * (a->d / VE);
     MM_CHECK(items < (1LL << 31), "paged_cache_fill: too many tokens for one call");
     const dim3 grid((unsigned)cdiv(items, 256), (unsigned)a->B);
     hipStream_t st = (hipStream_t)stream;
-#define MM_FILL(T_, VE_, PV_) hipLaunchKernelGGL((paged_fill_k<T_, VE_, PV_>), grid, dim3(256), 0, st, p)
-    if (a->dtype == MM_BF16) {
-        if (wide && pv) MM_FILL(bf16, 8, true); else if (wide) MM_FILL(bf16, 8, false); else MM_FILL(bf16, 1, true);
-    } else {
-        if (wide && pv) MM_FILL(float, 4, true); else if (wide) MM_FILL(float, 4, false); else MM_FILL(float, 1, true);
-    }
-#undef MM_FILL
+    if (a->dtype == MM_F32) hipLaunchKernelGGL((paged_fill_k<float, 4>), grid, dim3(256), 0, st, p);
+    else if (VE == 8) hipLaunchKernelGGL((paged_fill_k<bf16, 8>), grid, dim3(256), 0, st, p);
+    else hipLaunchKernelGGL((paged_fill_k<bf16, 4>), grid, dim3(256), 0, st, p);
     MM_LAUNCH_CHECK();
     return MM_OK;
 }
