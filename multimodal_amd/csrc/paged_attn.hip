@@ -82,30 +82,38 @@ template <typename T, int VE> __device__ __forceinline__ void raw_piece(const T*
 #pragma unroll
         for (int e = 0; e < VE; e++) v[e] = c + e < d ? to_f(x[c + e]) : 0.f;
 }
-// values c .. c + VE - 1 of a row, v, rotated (half layout over the first rot values) at the table row cs / sn
-template <typename T, int VE> __device__ __forceinline__ void turn(const T* x, int c, int rot, const float* cs, const float* sn, float (&v)[VE]) {
-    if (c >= rot) return;
-    const int half = rot >> 1;
-    const bool low = c < half;
-    if (low ? c + VE <= half : c + VE <= rot) {                                // within one half: partners and angles are consecutive too
-        const int i = low ? c : c - half;
-        float o[VE], cv[VE], sv[VE];
-        load_any(x + (low ? c + half : i), o);
-        load_any(cs + i, cv);
-        load_any(sn + i, sv);
-#pragma unroll
-        for (int e = 0; e < VE; e++) v[e] = low ? fmaf(v[e], cv[e], -(o[e] * sv[e])) : fmaf(v[e], cv[e], o[e] * sv[e]);
-        return;
-    }
-#pragma unroll
-    for (int e = 0; e < VE; e++)
-        if (c + e < rot) {
-            const bool first = c + e < half;
-            const int i = first ? c + e : c + e - half;
-            const float o = to_f(x[first ? c + e + half : i]);
-            v[e] = first ? fmaf(v[e], cs[i], -(o * sn[i])) : fmaf(v[e], cs[i], o * sn[i]);
+// what rotates the values c .. c + VE - 1 of a row (half layout over its first rot values): partners and angles
+template <typename T, int VE> struct Turn {
+    float o[VE], cv[VE], sv[VE];
+    bool low;
+    int n;                                                                     // how many of the values are rotated
+    // cs / sn: the tables' row of the position
+    __device__ __forceinline__ void load(const T* x, int c, int rot, const float* cs, const float* sn) {
+        n = min(max(rot - c, 0), VE);
+        if (n == 0) return;
+        const int half = rot >> 1;
+        low = c < half;
+        if (low ? c + VE <= half : c + VE <= rot) {                            // within one half: partners and angles are consecutive too
+            const int i = low ? c : c - half;
+            load_any(x + (low ? c + half : i), o);
+            load_any(cs + i, cv);
+            load_any(sn + i, sv);
+            return;
         }
-}
+#pragma unroll
+        for (int e = 0; e < VE; e++) {
+            const bool first = c + e < half;
+            const int i = c + e >= rot ? 0 : first ? c + e : c + e - half;
+            o[e] = to_f(x[first ? i + half : i]);
+            if (first != low) o[e] = -o[e];
+            cv[e] = cs[i]; sv[e] = sn[i];
+        }
+    }
+    __device__ __forceinline__ void apply(float (&v)[VE]) const {
+#pragma unroll
+        for (int e = 0; e < VE; e++) v[e] = e < n ? fmaf(v[e], cv[e], low ? -(o[e] * sv[e]) : o[e] * sv[e]) : v[e];
+    }
+};
 // stablemax's s(x); the reciprocal is within one unit in the last place
 __device__ __forceinline__ float stable_s(float x) { return x < 0.f ? __builtin_amdgcn_rcpf(1.f - x + 1e-9f) : x + 1.f; }
 
@@ -385,46 +393,44 @@ __global__ __launch_bounds__(256, (VE * NS * sizeof(T) * NT <= 32 ? 3 : VE * NS 
         }
         st.load_v(vp, vrow, d, li);
     };
-    Pages e0, e1;
-    int s0 = lo + wave * SL;
-    const bool any = s0 < hi;                                                           // wave-uniform
-    if (any) {
-        fetch(s0, e0);
-        fetch(s0 + RD, e1);
-        load_k(s0, e0);
-        load_v(s0, e0);
-    }
-    // ---- q (and the new key), rotated, while the first rows are under way
+    // ---- q (and the new key), rotated: loaded beside the page numbers, which the cache's rows wait for, and stored while those are under way
+    // (loaded behind the rows it came after them).  Columns past d are zero, as in trim_k.
+    constexpr int PE = S_t::PE, PIECES = DP / PE;
     const long trow = (long)paged_pos(p.positions, p.lengths, p.kn != nullptr, p.n_pos, b) * (p.rot >> 1);
     const float* cs = p.cos_t + trow; const float* sn = p.sin_t + trow;
-    constexpr int PE = S_t::PE, PIECES = DP / PE;                                       // columns past d: zero, as in trim_k
-    for (int i = tid; i < nh * PIECES; i += TT) {
+    const int pieces = (nh + (mine ? 1 : 0)) * PIECES;                                  // the new key: behind the last head
+    struct Item { float x[PE], y[PE]; Turn<T, PE> turn; };
+    auto take = [&](int i, Item& t) {
         const int h = i / PIECES, c = i % PIECES * PE;
-        float x[PE];
-        const T* row = (const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d;
-        raw_piece(row, c, d, x);
-        turn(row, c, p.rot, cs, sn, x);
-        S_t::put_q(qlds, HEADS, h, c, x);
-    }
-    if (mine)
-        for (int i = tid; i < PIECES; i += TT) {
-            const int c = i * PE;
-            float x[PE], y[PE];
-            const T* row = (const T*)p.kn + (long)b * p.ld_k + (long)hk * d;
-            raw_piece(row, c, d, x);
-            turn(row, c, p.rot, cs, sn, x);
-            raw_piece((const T*)p.vn + (long)b * p.ld_v + (long)hk * d, c, d, y);
-            VecIO<T, PE>::store(own_k + c, x); VecIO<T, PE>::store(own_v + c, y);       // the key rounded to the cache's type, as it is stored
-            if (own_row >= 0 && ct == 0) {
-                T* kd = (T*)p.kpool + own_row * d + c; T* vd = (T*)p.vpool + own_row * d + c;
+        const T* row = h < nh ? (const T*)p.q + (long)b * p.ld_q + (long)(h0 + h) * d : (const T*)p.kn + (long)b * p.ld_k + (long)hk * d;
+        raw_piece(row, c, d, t.x);
+        t.turn.load(row, c, p.rot, cs, sn);
+        if (h == nh) raw_piece((const T*)p.vn + (long)b * p.ld_v + (long)hk * d, c, d, t.y);
+    };
+    auto put = [&](int i, Item& t) {
+        const int h = i / PIECES, c = i % PIECES * PE;
+        t.turn.apply(t.x);
+        if (h < nh) { S_t::put_q(qlds, HEADS, h, c, t.x); return; }
+        VecIO<T, PE>::store(own_k + c, t.x); VecIO<T, PE>::store(own_v + c, t.y);       // the key rounded to the cache's type, as it is stored
+        if (own_row >= 0 && ct == 0) {
+            T* kd = (T*)p.kpool + own_row * d + c; T* vd = (T*)p.vpool + own_row * d + c;
 #pragma unroll
-                for (int e = 0; e < PE; e += 4)
-                    if (c + e < d) {
-                        const float a[4] = {x[e], x[e + 1], x[e + 2], x[e + 3]}, w[4] = {y[e], y[e + 1], y[e + 2], y[e + 3]};
-                        VecIO<T, 4>::store(kd + e, a); VecIO<T, 4>::store(vd + e, w);
-                    }
-            }
+            for (int e = 0; e < PE; e += 4)
+                if (c + e < d) {
+                    const float a[4] = {t.x[e], t.x[e + 1], t.x[e + 2], t.x[e + 3]}, w[4] = {t.y[e], t.y[e + 1], t.y[e + 2], t.y[e + 3]};
+                    VecIO<T, 4>::store(kd + e, a); VecIO<T, 4>::store(vd + e, w);
+                }
         }
+    };
+    Pages e0, e1;
+    Item item;
+    int s0 = lo + wave * SL;
+    const bool any = s0 < hi;                                                           // wave-uniform
+    if (any) { fetch(s0, e0); fetch(s0 + RD, e1); }
+    if (tid < pieces) take(tid, item);
+    if (any) { load_k(s0, e0); load_v(s0, e0); }
+    if (tid < pieces) put(tid, item);
+    for (int i = tid + TT; i < pieces; i += TT) { take(i, item); put(i, item); }
     sync();
     const T* q = qlds + min(li, nh - 1) * S_t::QS + g * S_t::PE;                        // columns past the last head repeat it; nothing reads them
 
@@ -785,7 +791,9 @@ template <typename T, int VE> __global__ __launch_bounds__(256) void paged_fill_
     if (c < p.rot) {
         const long pos = p.positions ? (long)p.positions[b] + s : (long)st + s;
         const long t = min(max(pos, 0L), (long)p.n_pos - 1) * (p.rot >> 1);
-        turn(k, c, p.rot, p.cos_t + t, p.sin_t + t, x);
+        Turn<T, VE> turn;
+        turn.load(k, c, p.rot, p.cos_t + t, p.sin_t + t);
+        turn.apply(x);
     }
     const long row = p.map.row(b, h, st + s);
     if (row < 0) return;
