@@ -2,9 +2,11 @@
 //
 // Per (row, KV head): the A = budget - recent greatest of `old` weights, then as few moves as possible.  Attention does not ask for an
 // order of the slots, so survivors among the first A slots stay; the i-th hole there takes the i-th survivor from behind.  Sources (>= A)
-// and targets (< A) are disjoint: all moves are independent.  The newest slots then shift down by n - budget; a slot's target is the
+// and targets (< A) are disjoint: all moves are independent.  The newest slots shift down by n - budget; a slot's target is the
 // source of the slot n - budget before it, so the slots of one residue class mod n - budget form a chain, and a thread that walks its
-// chain in order needs no one else.  HBM bounds the moves: 4 d values per slot moved (K and V, read and written).
+// chain in order needs no one else.  Of the survivors only those in slots that the shift overwrites are in its way: the first slot of a chain,
+// which its walker moves before it begins.  So moves and shift are one launch.  HBM bounds it: 4 d values per slot moved (K and V, read and
+// written).
 //
 // Selection: weights as ordered 32-bit keys, the A-th greatest found bit by bit from the top: count the keys >= candidate by ballots
 // (no atomics: a histogram's bins collide where weights are alike, and equal weights are the rule at the start).  Up to 65536 slots stay
@@ -19,11 +21,13 @@ __device__ __forceinline__ unsigned weight_key(float x) {
 }
 struct EvictP {
     char* kpool; char* vpool; float* w; int* lengths; int* kept; PagedMap map;
-    char* ws; int room;            // per (row, KV head): {slots, moves}; pool rows to [room] and from [room] of the moves; the same as slots
+    char* ws; int room;            // per (row, KV head): {slots, moves, of them by the shift}; pool rows to [room] and from [room] of the moves;
+                                   // where the shift moves what it finds, pool rows [recent] or -1; the moves as slots (without a room none of them)
     int units, budget, recent;                                                 // units: 16- or 8-byte pieces of a slot's K
-    __device__ __forceinline__ int* head(long bh) const { return (int*)(ws + bh * (24L * room + 16)); }
+    __device__ __forceinline__ int* head(long bh) const { return (int*)(ws + bh * (24L * room + (room ? 8L * recent : 0) + 16)); }
     __device__ __forceinline__ long* rows(long bh) const { return (long*)(head(bh) + 4); }
-    __device__ __forceinline__ int* slots(long bh) const { return (int*)(rows(bh) + 2L * room); }
+    __device__ __forceinline__ long* dest(long bh) const { return rows(bh) + 2L * room; }
+    __device__ __forceinline__ int* slots(long bh) const { return (int*)(dest(bh) + recent); }
 };
 
 // ------------------------------------------------------------------------------------------------ selection (NW waves)
@@ -52,14 +56,14 @@ template <int NW> __device__ __forceinline__ int block_scan(int v, int* red, int
     return before + s - v;
 }
 
-// R registers of keys a thread (four consecutive slots a round), R = 0: read again in every pass
-template <int NW, int R> __device__ __forceinline__ void evict_select(const EvictP& p, int b, int h, int* red) {
+// R registers of keys a thread (four consecutive slots a round), R = 0: read again in every pass.  SPLIT: moves and shift run side by side
+template <int NW, int R, bool SPLIT> __device__ __forceinline__ void evict_select(const EvictP& p, int b, int h, int* red) {
     constexpr int ROUND = NW * 256;
     const long bh = (long)b * p.map.Hkv + h;
     const int tid = threadIdx.x, n = min(p.lengths[b], p.map.capacity());
     int* kept = p.kept + bh * p.budget;
     int* hd = p.head(bh);
-    if (tid == 0) { hd[0] = n; hd[1] = 0; }
+    if (tid == 0) { hd[0] = n; hd[1] = 0; hd[2] = 0; }
     if (n <= p.budget) return;
     const int A = p.budget - p.recent, old = n - p.recent, rounds = (old + ROUND - 1) / ROUND;
     // the moves as slots: in LDS where they fit (at most half of the slots move)
@@ -144,11 +148,11 @@ template <int NW, int R> __device__ __forceinline__ void evict_select(const Evic
         for (int r = 0; r < RR; r++) if (r < rounds) place(r, key[r]);
     } else
         for (int r = 0; r < rounds; r++) { unsigned k[4]; load(r, k); place(r, k); }
-    for (int j = A + tid; j < p.budget; j += NW * 64) kept[j] = n - p.budget + j;
+    long* rows = p.rows(bh); long* dest = p.dest(bh);                          // looked up once here, not once a piece
+    for (int j = A + tid; j < p.budget; j += NW * 64) { kept[j] = n - p.budget + j; if (SPLIT && p.room) dest[j - A] = -1; }
     __syncthreads();                                                           // the lists are written
     const int moves = min(holes, late);
     if (tid == 0) hd[1] = moves;
-    long* rows = p.rows(bh);                                                   // looked up once here, not once a piece
     constexpr int N = 4;
     for (int i0 = tid; i0 < moves; i0 += NW * 64 * N) {
         int ts[N], fs[N];
@@ -165,17 +169,23 @@ template <int NW, int R> __device__ __forceinline__ void evict_select(const Evic
             if (ts[j] >= 0) {
                 const int i = i0 + j * NW * 64;
                 kept[ts[j]] = fs[j];
-                rows[i] = rf[j] < 0 ? -1 : rt[j]; rows[p.room + i] = rf[j];
+                if (rf[j] < 0) rt[j] = -1;
+                rows[i] = rt[j]; rows[p.room + i] = rf[j];
+                if (SPLIT && fs[j] < p.budget) {                                   // sources ascend: these are the first moves
+                    dest[fs[j] - A] = rt[j];
+                    if (i + 1 == moves || from[i + 1] >= p.budget) hd[2] = i + 1;
+                }
             }
     }
 }
 
 // ------------------------------------------------------------------------------------------------ moving
-// independent moves [first, ..) of a (row, KV head), one piece of K and of V a thread; `step` threads share the work
+// the moves of a (row, KV head) that the shift does not make, one piece of K and of V a thread; `step` threads share the work
 template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& p, int b, int h, int t, int step) {
     const long bh = (long)b * p.map.Hkv + h;
-    const long* to = p.rows(bh); const long* from = to + p.room;
-    const unsigned total = (unsigned)p.head(bh)[1] * (unsigned)p.units;
+    const int first = p.head(bh)[2];
+    const long* to = p.rows(bh) + first; const long* from = to + p.room;
+    const unsigned total = (unsigned)(p.head(bh)[1] - first) * (unsigned)p.units;
     U* K = (U*)p.kpool; U* V = (U*)p.vpool;
     constexpr int N = 4;                                                       // in flight
     for (unsigned i0 = t; i0 < total; i0 += (unsigned)step * N) {
@@ -207,13 +217,14 @@ template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& 
     }
 }
 // The newest slots, down by n - budget, by `blocks` workgroups of NT threads: a chain (residue class) and piece a thread where there are enough
-// of them.  Few chains are long ones (one token over the budget: one chain of all the newest slots): then one workgroup moves tile
+// of them.  The survivor in a chain's first slot goes to its hole first.  Few chains are long ones (one token over the budget: one chain of all the newest slots): then one workgroup moves tile
 // after tile instead, all loads of a tile before its stores, which only overwrite what has been loaded (96 heads of 964 newest slots, some
 // rows one slot over: 550 us in chains).
-template <typename U, int NT> __device__ __forceinline__ void evict_shift(const EvictP& p, int b, int h, int block, int blocks) {
+template <typename U, int NT, bool SPLIT> __device__ __forceinline__ void evict_shift(const EvictP& p, int b, int h, int block, int blocks) {
     const int n = p.head((long)b * p.map.Hkv + h)[0];
     if (n <= p.budget || !p.recent) return;
     const int by = n - p.budget, first = n - p.recent, tid = threadIdx.x;
+    const long* dest = p.dest((long)b * p.map.Hkv + h);
     const unsigned total = (unsigned)min(by, p.recent) * (unsigned)p.units, all = (unsigned)p.recent * (unsigned)p.units;
     U* K = (U*)p.kpool; U* V = (U*)p.vpool;
     constexpr int N = 4;
@@ -231,21 +242,41 @@ template <typename U, int NT> __device__ __forceinline__ void evict_shift(const 
         K[d * p.units + piece] = k; V[d * p.units + piece] = v;
         if (piece == 0) p.w[d] = w;
     };
+    auto clear = [&](int c, int piece, long& d, U& k, U& v, float& w) {        // the survivor in the first slot of chain c
+        d = SPLIT && p.room ? dest[c] : -1;
+        if (d < 0) return;
+        const long s = p.map.row(b, h, first + c - by);
+        k = K[s * p.units + piece]; v = V[s * p.units + piece];
+        if (piece == 0) w = p.w[s];
+    };
     if (total >= all || total >= NT / 2) {
         for (unsigned i = (unsigned)(block * NT + tid); i < total; i += (unsigned)(blocks * NT)) {
             const unsigned c = i / (unsigned)p.units;
             const int piece = (int)(i - c * (unsigned)p.units);
+            U k0, v0;
+            float w0;
+            long d0;
+            clear((int)c, piece, d0, k0, v0, w0);
             for (long j0 = c; j0 < p.recent; j0 += (long)N * by) {
                 U k[N], v[N];
                 float w[N];
                 long d[N];
 #pragma unroll
                 for (int e = 0; e < N; e++) { const long j = j0 + (long)e * by; d[e] = -1; if (j < p.recent) take(j, piece, d[e], k[e], v[e], w[e]); }
+                if (j0 == c) put(piece, d0, k0, v0, w0);
 #pragma unroll
                 for (int e = 0; e < N; e++) put(piece, d[e], k[e], v[e], w[e]);
             }
         }
     } else if (block == 0) {
+        if ((unsigned)tid < total) {
+            const int c = tid / p.units, piece = tid - c * p.units;
+            U k0, v0;
+            float w0;
+            long d0;
+            clear(c, piece, d0, k0, v0, w0);
+            put(piece, d0, k0, v0, w0);
+        }
         for (unsigned i0 = 0; i0 < all; i0 += NT * N) {
             U k[N], v[N];
             float w[N];
@@ -266,6 +297,7 @@ template <typename U, int NT> __device__ __forceinline__ void evict_shift(const 
 }
 
 // ------------------------------------------------------------------------------------------------ kernels
+constexpr int MOVERS = 1024;                                                   // 512: few long chains 50 us for 40 (12 rows of 8 heads of 964 newest slots)
 // A workgroup per (row, KV head).  ALL: it moves and shifts as well.
 template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW * 64) void evict_select_k(const EvictP p) {
     __shared__ int red[2 * NW];
@@ -274,24 +306,22 @@ template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW *
         int* kept = p.kept + ((long)b * p.map.Hkv + h) * p.budget;
         for (int j = threadIdx.x; j < p.budget; j += NW * 64) kept[j] = j < n ? j : -1;
     }
-    evict_select<NW, R>(p, b, h, red);
+    evict_select<NW, R, !ALL>(p, b, h, red);
     if constexpr (ALL) {
         __syncthreads();
         evict_moves<U>(p, b, h, threadIdx.x, NW * 64);
         __syncthreads();                                                       // targets of the shift were sources of the moves
-        evict_shift<U, NW * 64>(p, b, h, 0, 1);
+        evict_shift<U, NW * 64, false>(p, b, h, 0, 1);
     }
 }
-// The last launch writes the new lengths: only the selection reads the old ones.
+// Only the selection reads the old lengths.
 __device__ __forceinline__ void evict_length(const EvictP& p, int b) {
     if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.head((long)b * p.map.Hkv)[0] > p.budget) p.lengths[b] = p.budget;
 }
-template <typename U, bool LAST> __global__ __launch_bounds__(256) void evict_moves_k(const EvictP p) {
-    evict_moves<U>(p, blockIdx.x, blockIdx.y, blockIdx.z * 256 + threadIdx.x, gridDim.z * 256);
-    if constexpr (LAST) evict_length(p, blockIdx.x);
-}
-template <typename U> __global__ __launch_bounds__(1024) void evict_shift_k(const EvictP p) {
-    evict_shift<U, 1024>(p, blockIdx.x, blockIdx.y, blockIdx.z, gridDim.z);
+// shifters workgroups of each (row, KV head) shift, the others move
+template <typename U> __global__ __launch_bounds__(MOVERS) void evict_move_k(const EvictP p, int shifters) {
+    if ((int)blockIdx.z < shifters) evict_shift<U, MOVERS, true>(p, blockIdx.x, blockIdx.y, blockIdx.z, shifters);
+    else evict_moves<U>(p, blockIdx.x, blockIdx.y, (blockIdx.z - shifters) * MOVERS + threadIdx.x, (gridDim.z - shifters) * MOVERS);
     evict_length(p, blockIdx.x);
 }
 __global__ __launch_bounds__(64) void evict_lengths_k(const EvictP p) { evict_length(p, blockIdx.x); }
@@ -302,14 +332,15 @@ static int64_t evict_room(int64_t page, int64_t width, int64_t budget, int64_t r
 }
 extern "C" size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page, int64_t width, int64_t budget, int64_t recent) {
     if (B <= 0 || Hkv <= 0 || page <= 0 || width <= 0 || recent < 0 || budget < recent) return 0;
-    return (size_t)(B * Hkv) * (size_t)(24 * evict_room(page, width, budget, recent) + 16);
+    const int64_t room = evict_room(page, width, budget, recent);
+    return (size_t)(B * Hkv) * (size_t)(24 * room + (room ? 8 * recent : 0) + 16);
 }
 
 template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64_t cap, hipStream_t st) {
     const dim3 grid((unsigned)B, (unsigned)p.map.Hkv);
     const int64_t heads = B * p.map.Hkv;
     // One workgroup does everything where there is little to move; else the moves and the shift spread over the card in launches of their
-    // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 181 in three).
+    // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 178 in two; 181 with the shift in a third).
     const bool all = ((int64_t)p.room + p.recent) * p.units <= 8192;
 #define MM_SELECT(NW_, R_) do { if (all) hipLaunchKernelGGL((evict_select_k<NW_, R_, U, true>), grid, dim3(NW_ * 64), 0, st, p); \
                                      else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
@@ -319,18 +350,13 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
     else if (cap <= 65536) MM_SELECT(16, 64);
     else MM_SELECT(16, 0);
 #undef MM_SELECT
-    auto split = [&](int64_t items) {                                          // workgroups per (row, KV head): four pieces a thread, 4096 workgroups in all
-        const int64_t w = cdiv(items, 1024), most = cdiv(4096, heads);
-        return (unsigned)(w < 1 ? 1 : w < most ? w : most);
+    auto split = [&](int64_t items, int64_t each, int64_t in_all) {            // workgroups per (row, KV head), `each` pieces a thread where they suffice
+        const int64_t w = cdiv(items, MOVERS * each), most = cdiv(in_all, heads);
+        return (unsigned)(w < most ? w : most);
     };
-    if (!all && p.room) {
-        const dim3 g(grid.x, grid.y, split((int64_t)p.room * p.units));
-        if (p.recent) hipLaunchKernelGGL((evict_moves_k<U, false>), g, dim3(256), 0, st, p);
-        else hipLaunchKernelGGL((evict_moves_k<U, true>), g, dim3(256), 0, st, p);
-    }
-    if (!all && p.recent) {
-        const int64_t w = cdiv((int64_t)p.recent * p.units, 1024), most = cdiv(2048, heads);   // a piece a thread
-        hipLaunchKernelGGL(evict_shift_k<U>, dim3(grid.x, grid.y, (unsigned)(w < 1 ? 1 : w < most ? w : most)), dim3(1024), 0, st, p);
+    if (!all) {
+        const unsigned shifters = split((int64_t)p.recent * p.units, 1, 4096), movers = split((int64_t)p.room * p.units, 4, 2048);
+        hipLaunchKernelGGL(evict_move_k<U>, dim3(grid.x, grid.y, shifters + movers), dim3(MOVERS), 0, st, p, (int)shifters);
     }
     if (all) hipLaunchKernelGGL(evict_lengths_k, dim3(grid.x), dim3(64), 0, st, p);
 }
