@@ -245,7 +245,8 @@ int mm_orthograd_adamw_dev(const mm_param_desc* descs, const int32_t* chunk_tens
  *   weights:      float [n_pages][Hkv][page] or NULL: the attention weight each slot has drawn so far.
  * A slot whose page number is outside [0, n_pages) or whose index is not below width * page does not exist: it is neither
  * read nor written, and attention passes it over.  Pages that a call writes (k_new / v_new, weights, fill, evict) belong to
- * one row alone; pages that are only read may be shared by rows (a common prompt).  Page offsets are 64-bit. */
+ * one row alone; pages that are only read may be shared by rows (a common prompt).  A length beyond width * page counts as
+ * width * page.  Page offsets are 64-bit. */
 typedef struct {
     const void* q;              /* [B][H][d], row stride ld_q */
     const void* k_new;          /* [B][Hkv][d], row stride ld_k; NULL: attend from what is stored, append nothing */
@@ -265,8 +266,8 @@ typedef struct {
 } mm_paged_attn_args;
 /* One token of every row: q and k_new are rotated (half layout, first rot dims) at the row's position, k_new (rotated, rounded to
  * the cache's type) and v_new are stored at slot lengths[b], and q attends over slots 0 .. lengths[b] (over 0 .. lengths[b] - 1
- * without k_new).  lengths is not changed.  A row without a slot, and one whose scores are all -inf, gets o = 0.  Scores, softmax statistics, sums and weights are
- * float32; results do not depend on what else runs (no atomics). */
+ * without k_new).  lengths is not changed.  A row without a slot, and one whose scores are all -inf, gets o = 0.  Scores,
+ * softmax statistics, sums and weights are float32; results do not depend on what else runs (no atomics). */
 size_t mm_paged_decode_attn_workspace(const mm_paged_attn_args* args);
 int mm_paged_decode_attn(const mm_paged_attn_args* args, void* stream);
 

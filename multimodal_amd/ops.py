@@ -465,7 +465,8 @@ def paged_decode_attn(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor
     of drafted tokens stored by paged_cache_fill: one row per token, the table's row repeated).  positions int32 [B]: the rotary
     position where it is not the slot (after paged_evict).  weights float32 [pages, Hkv, page]: accumulates the attention each slot
     draws (paged_evict goes by it).  A row with lengths < 0 sits out; a row without a slot, and one that sits out, gets zeros.  A token
-    whose page the table does not hold is neither stored nor attended.  Pages written by a call belong to one row.  Returns o [B, H*d]."""
+    whose page the table does not hold is neither stored nor attended.  Pages written by a call belong to one row, with weights all that
+    it attends over.  Returns o [B, H*d]."""
     who = "paged_decode_attn"
     dev, code, B, n_pages, Hkv, page, d, width, ld_table = _cache_geom(who, kpool, vpool, page_table, weights)
     if H <= 0 or H % Hkv:

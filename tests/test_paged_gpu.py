@@ -646,6 +646,42 @@ def test_evict_pages_the_table_does_not_hold():
     assert kept[1, 0].tolist() == _evict_reference(ws[1].tolist(), 160, 60, 12)
 
 
+def test_evict_many_slots_and_missing_pages():
+    """Moves and shift side by side, with pages missing among the holes, the survivors, the slots the shift overwrites and those it takes: what has
+    a source and a target moves, everything else stays."""
+    from multimodal_amd import ops
+    n_slots, budget, recent, page, d = [4000, 2300], 2000, 600, 16, 128
+    g = torch.Generator().manual_seed(44)
+    c = Cache(44, torch.bfloat16, 2, 2, d, page, n_slots, weights=True, garbage=0.0)
+    ws = []
+    for b, n in enumerate(n_slots):
+        w = torch.rand(2, n, generator=g) + 0.5
+        c.put(c.k, b, n, _randn(g, 2, n, d)); c.put(c.v, b, n, _randn(g, 2, n, d)); c.put(c.w, b, n, w)
+        ws.append(w)
+    for b, entry in ((0, 4), (0, 88), (0, 110), (0, 150), (0, 225), (1, 3), (1, 90), (1, 107), (1, 130)):
+        c.table[b, entry] = -1 if entry % 2 else c.n_pages
+        s = slice(entry * page, (entry + 1) * page)
+        ws[b][:, s] = -math.inf
+    before = (c.k.clone(), c.v.clone(), c.w.clone())
+    n_dev = torch.tensor(n_slots, dtype=torch.int32, device=DEV)
+    kept = ops.paged_evict(c.k, c.v, c.w, c.table, n_dev, budget, recent)
+    assert n_dev.tolist() == [budget, budget]
+    want = [x.clone() for x in before]
+    table = c.table.cpu().long()
+    for b, n in enumerate(n_slots):
+        for h in range(2):
+            ref = _evict_reference(ws[b][h].tolist(), n, budget, recent)
+            assert kept[b, h].tolist() == ref, (b, h)
+            src, to = torch.tensor(ref), torch.arange(budget)
+            ps, pt = table[b][src // page], table[b][to // page]
+            both = (ps >= 0) & (ps < c.n_pages) & (pt >= 0) & (pt < c.n_pages)
+            ps, pt, os, ot = ps[both].to(DEV), pt[both].to(DEV), (src % page)[both].to(DEV), (to % page)[both].to(DEV)
+            for x, y in zip(want, before):
+                x[pt, h, ot] = y[ps, h, os]
+    for x, y in zip((c.k, c.v, c.w), want):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
 # ------------------------------------------------------------------------------------------------ together
 def _simulate(dtype, lens, steps, budget, recent, stable, seed=50):
     """Prompts, steps with weights, an eviction whenever a row passes its budget: the operators against a 64-bit simulation that keeps each row's
