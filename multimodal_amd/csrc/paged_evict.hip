@@ -180,8 +180,9 @@ template <int NW, int R, bool SPLIT> __device__ __forceinline__ void evict_selec
 }
 
 // ------------------------------------------------------------------------------------------------ moving
-// the moves of a (row, KV head) that the shift does not make, one piece of K and of V a thread; `step` threads share the work
-template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& p, int b, int h, int t, int step) {
+// the moves of a (row, KV head) that the shift does not make, one piece of K and of V a thread; `step` threads share the work.
+// ST: past the last-level cache (non-temporal)
+template <typename U, bool ST> __device__ __forceinline__ void evict_moves(const EvictP& p, int b, int h, int t, int step) {
     const long bh = (long)b * p.map.Hkv + h;
     const int first = p.head(bh)[2];
     const long* to = p.rows(bh) + first; const long* from = to + p.room;
@@ -203,7 +204,8 @@ template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& 
                 const long s = from[m];
                 d[j] = to[m];
                 if (d[j] >= 0) {
-                    k[j] = K[s * p.units + piece[j]]; v[j] = V[s * p.units + piece[j]];
+                    const U* ks = K + s * p.units + piece[j]; const U* vs = V + s * p.units + piece[j];
+                    k[j] = ST ? __builtin_nontemporal_load(ks) : *ks; v[j] = ST ? __builtin_nontemporal_load(vs) : *vs;
                     if (piece[j] == 0) w[j] = p.w[s];
                 }
             }
@@ -211,7 +213,9 @@ template <typename U> __device__ __forceinline__ void evict_moves(const EvictP& 
 #pragma unroll
         for (int j = 0; j < N; j++)
             if (d[j] >= 0) {
-                K[d[j] * p.units + piece[j]] = k[j]; V[d[j] * p.units + piece[j]] = v[j];
+                U* kd = K + d[j] * p.units + piece[j]; U* vd = V + d[j] * p.units + piece[j];
+                if constexpr (ST) { __builtin_nontemporal_store(k[j], kd); __builtin_nontemporal_store(v[j], vd); }
+                else { *kd = k[j]; *vd = v[j]; }
                 if (piece[j] == 0) p.w[d[j]] = w[j];
             }
     }
@@ -309,7 +313,7 @@ template <int NW, int R, typename U, bool ALL> __global__ __launch_bounds__(NW *
     evict_select<NW, R, !ALL>(p, b, h, red);
     if constexpr (ALL) {
         __syncthreads();
-        evict_moves<U>(p, b, h, threadIdx.x, NW * 64);
+        evict_moves<U, false>(p, b, h, threadIdx.x, NW * 64);
         __syncthreads();                                                       // targets of the shift were sources of the moves
         evict_shift<U, NW * 64, false>(p, b, h, 0, 1);
     }
@@ -319,9 +323,9 @@ __device__ __forceinline__ void evict_length(const EvictP& p, int b) {
     if (blockIdx.y == 0 && blockIdx.z == 0 && threadIdx.x == 0 && p.head((long)b * p.map.Hkv)[0] > p.budget) p.lengths[b] = p.budget;
 }
 // shifters workgroups of each (row, KV head) shift, the others move
-template <typename U> __global__ __launch_bounds__(MOVERS) void evict_move_k(const EvictP p, int shifters) {
+template <typename U, bool ST> __global__ __launch_bounds__(MOVERS) void evict_move_k(const EvictP p, int shifters) {
     if ((int)blockIdx.z < shifters) evict_shift<U, MOVERS, true>(p, blockIdx.x, blockIdx.y, blockIdx.z, shifters);
-    else evict_moves<U>(p, blockIdx.x, blockIdx.y, (blockIdx.z - shifters) * MOVERS + threadIdx.x, (gridDim.z - shifters) * MOVERS);
+    else evict_moves<U, ST>(p, blockIdx.x, blockIdx.y, (blockIdx.z - shifters) * MOVERS + threadIdx.x, (gridDim.z - shifters) * MOVERS);
     evict_length(p, blockIdx.x);
 }
 __global__ __launch_bounds__(64) void evict_lengths_k(const EvictP p) { evict_length(p, blockIdx.x); }
@@ -340,7 +344,7 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
     const dim3 grid((unsigned)B, (unsigned)p.map.Hkv);
     const int64_t heads = B * p.map.Hkv;
     // One workgroup does everything where there is little to move; else the moves and the shift spread over the card in launches of their
-    // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 178 in two; 181 with the shift in a third).
+    // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 170 in two).
     const bool all = ((int64_t)p.room + p.recent) * p.units <= 8192;
 #define MM_SELECT(NW_, R_) do { if (all) hipLaunchKernelGGL((evict_select_k<NW_, R_, U, true>), grid, dim3(NW_ * 64), 0, st, p); \
                                      else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
@@ -355,8 +359,12 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
         return (unsigned)(w < most ? w : most);
     };
     if (!all) {
-        const unsigned shifters = split((int64_t)p.recent * p.units, 1, 4096), movers = split((int64_t)p.room * p.units, 4, 2048);
-        hipLaunchKernelGGL(evict_move_k<U>, dim3(grid.x, grid.y, shifters + movers), dim3(MOVERS), 0, st, p, (int)shifters);
+        const unsigned shifters = split((int64_t)p.recent * p.units, 2, 1024), movers = split((int64_t)p.room * p.units, 4, 2048);
+        const dim3 g(grid.x, grid.y, shifters + movers);
+        // Where the rows' slots are more than the last-level cache holds, what is moved goes past it (384 heads halved from up to 8192 slots of 512
+        // bytes: 170 us, 178 through it; 128 heads from 2000 to 1024, which it holds: 33 and 29).
+        if (heads * cap * p.units * (int64_t)sizeof(U) * 2 > (256LL << 20)) hipLaunchKernelGGL((evict_move_k<U, true>), g, dim3(MOVERS), 0, st, p, (int)shifters);
+        else hipLaunchKernelGGL((evict_move_k<U, false>), g, dim3(MOVERS), 0, st, p, (int)shifters);
     }
     if (all) hipLaunchKernelGGL(evict_lengths_k, dim3(grid.x), dim3(64), 0, st, p);
 }
