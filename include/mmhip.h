@@ -245,8 +245,8 @@ int mm_orthograd_adamw_dev(const mm_param_desc* descs, const int32_t* chunk_tens
  *   weights:      float [n_pages][Hkv][page] or NULL: the attention weight each slot has drawn so far.
  * A slot whose page number is outside [0, n_pages) or whose index is not below width * page does not exist: it is neither
  * read nor written, and attention passes it over.  Pages that a call writes (k_new / v_new, weights, fill, evict) belong to
- * one row alone; pages that are only read may be shared by rows (a common prompt).  A length beyond width * page counts as
- * width * page.  Page offsets are 64-bit. */
+ * one row alone, at one place of its table; pages that are only read may be shared by rows (a common prompt).  A length
+ * beyond width * page counts as width * page.  Page offsets are 64-bit. */
 typedef struct {
     const void* q;              /* [B][H][d], row stride ld_q */
     const void* k_new;          /* [B][Hkv][d], row stride ld_k; NULL: attend from what is stored, append nothing */

@@ -18,9 +18,9 @@
 // are split over workgroups and a second kernel joins them (and adds the weights up).  The token's own key and value are taken
 // from the inputs, not from the cache, so nothing waits for the append.  In a step's turn the next step's K is on its way while the
 // softmax runs, and its V once this V has been used: 8 to 16 KB a wave, 8 to 12 waves a CU.
-// Measured (a large copy: 5.1 TB/s): 1024 rows of 160 to 238 slots, 8 heads of 128, bf16: 849 MB in 152 us = 5.6 TB/s; 256 rows of 1000 to
+// Measured (a large copy: 5.1 TB/s): 1024 rows of 160 to 238 slots, 8 heads of 128, bf16: 849 MB in 150 us = 5.7 TB/s; 256 rows of 1000 to
 // 2000: 6.1 TB/s; 32 rows of 300 to 16384, 8 KV heads shared by 4: 188 us = 5.8 TB/s, with weights 248 (scores and weights are
-// another 90 MB); one row of 65551, 4 KV heads shared by 8: 37 us = 3.6 TB/s (two launches); float32, 64 rows of 1000 to 2000: 5.5 TB/s.
+// another 90 MB); one row of 65551, 4 KV heads shared by 8: 36 us = 3.7 TB/s (two launches); float32, 64 rows of 1000 to 2000: 5.5 TB/s.
 #include "paged.h"
 #include <type_traits>
 
