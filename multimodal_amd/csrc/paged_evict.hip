@@ -8,9 +8,12 @@
 // which its walker moves before it begins.  So moves and shift are one launch.  HBM bounds it: 4 d values per slot moved (K and V, read and
 // written).
 //
-// Selection: weights as ordered 32-bit keys, the A-th greatest found bit by bit from the top: count the keys >= candidate by ballots
-// (no atomics: a histogram's bins collide where weights are alike, and equal weights are the rule at the start).  Up to 65536 slots stay
-// in registers, longer rows are read again in every pass.
+// Selection: weights as ordered 32-bit keys, the A-th greatest found bit by bit, from the first bit in which they differ: count the keys
+// >= candidate by ballots (no histogram: its bins collide where weights are alike, and equal weights are the rule at the start).  Once at most
+// 64 keys are left in question each wave settles the rest alone (4 rows and heads of 40000 to 60000 slots, cut to 20000: 155 -> 136 us in all; of
+// 80000 to 100000: 486 -> 410).  Up to 65536 slots stay in registers, longer rows are read again in every pass.  384 heads of up to 8192
+// slots take 26 us: a workgroup loads for 3, counts for 8 (13 passes, each a barrier), settles the last 64 keys in 2, finds the places in 4 and the
+// moves' rows in 1; the rest is the launch and the longest rows.
 #include "paged.h"
 
 // Order of weights as unsigned integers: greater weight, greater key; NaN above everything, -0 = 0, a slot that does not exist lowest (0).
@@ -84,34 +87,77 @@ template <int NW, int R, bool SPLIT> __device__ __forceinline__ void evict_selec
 #pragma unroll
         for (int r = 0; r < RR; r++) load(r, key[r]);
     }
-    auto count = [&](unsigned t) {                                             // keys >= t (t > 0), over the wave
-        int c = 0;
+    auto each = [&](auto&& f) {                                                // f(round, its keys)
         if constexpr (R > 0) {
 #pragma unroll
-            for (int r = 0; r < RR; r++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) c += __popcll(__ballot(key[r][i] >= t));
-        } else {
-            for (int r = 0; r < rounds; r++) {
-                unsigned k[4];
-                load(r, k);
-#pragma unroll
-                for (int i = 0; i < 4; i++) c += __popcll(__ballot(k[i] >= t));
-            }
-        }
-        return c;
+            for (int r = 0; r < RR; r++) f(r, key[r]);
+        } else
+            for (int r = 0; r < rounds; r++) { unsigned k[4]; load(r, k); f(r, k); }
     };
-    int buf = 0, ge = old;                                                     // ge: keys >= T
+    auto count = [&](unsigned t) {                                             // keys >= t (t > 0), over the wave
+        int c = 0, all = 0;
+        if constexpr (R > 4) {                                                 // a lane's count first, its bits by ballots: fewer of them
+            each([&](int, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) c += k[i] >= t;
+            });
+#pragma unroll
+            for (int e = 0; 1 << e <= R; e++) all += __popcll(__ballot(c >> e & 1)) << e;
+        } else
+            each([&](int, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) all += __popcll(__ballot(k[i] >= t));
+            });
+        return all;
+    };
+    __shared__ unsigned ends[2 * NW], few[64];
+    __shared__ int nfew;
+    int buf = 0, ge = old, above = 0, bit = 31;                                // keys >= T; keys beyond those in question
+    int ties = 0x7fffffff;                                                     // how many keys equal to T are kept, lowest slots first
     unsigned T = 0;
     if (A == 0) { T = 0xffffffffu; ge = 0; }                                   // nothing of the old is kept
-    else
-        for (int bit = 31; bit >= 0 && ge != A; bit--) {
+    else {
+        if (tid == 0) nfew = 0;
+        if constexpr (R == 4) __syncthreads();
+        else {                                                                 // with few keys it costs more than the rounds it saves
+            unsigned top = 0, low = 0;                                         // greatest key, greatest complement
+            each([&](int r, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) if (r * ROUND + tid * 4 + i < old) { top = max(top, k[i]); low = max(low, ~k[i]); }
+            });
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) { top = max(top, (unsigned)__shfl_xor((int)top, o)); low = max(low, (unsigned)__shfl_xor((int)low, o)); }
+            if ((tid & 63) == 0) { ends[tid >> 6] = top; ends[NW + (tid >> 6)] = low; }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < NW; i++) { top = max(top, ends[i]); low = max(low, ends[NW + i]); }
+            const unsigned differ = top ^ ~low;
+            bit = differ ? 31 - __clz((int)differ) : -1;
+            T = bit == 31 ? 0u : top >> (bit + 1) << (bit + 1);
+        }
+        for (; bit >= 0 && ge != A && ge - above > 64; bit--) {
             const unsigned t = T | 1u << bit;
             const int c = block_count<NW>(count(t), red, buf);
-            if (c >= A) { T = t; ge = c; }
+            if (c >= A) { T = t; ge = c; } else above = c;
         }
-    int ties = 0x7fffffff;                                                     // how many keys equal to T are kept, lowest slots first
-    if (A && ge != A) ties = A - (T == 0xffffffffu ? 0 : block_count<NW>(count(T + 1), red, buf));
+        if (bit >= 0 && ge != A) {
+            const unsigned last = T | ((2u << bit) - 1u);
+            each([&](int r, const unsigned (&k)[4]) {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (k[i] >= T && k[i] <= last && r * ROUND + tid * 4 + i < old) few[atomicAdd(&nfew, 1)] = k[i];   // their order does not matter
+            });
+            __syncthreads();
+            const bool real = (tid & 63) < nfew;
+            const unsigned mine = real ? few[tid & 63] : 0u;
+            for (; bit >= 0 && ge != A; bit--) {
+                const unsigned t = T | 1u << bit;
+                const int c = above + __popcll(__ballot(real && mine >= t));
+                if (c >= A) { T = t; ge = c; }
+            }
+            if (ge != A) ties = A - above - __popcll(__ballot(real && mine > T));
+        } else if (ge != A) ties = A - (T == 0xffffffffu ? 0 : block_count<NW>(count(T + 1), red, buf));
+    }
     int equal = 0, holes = 0, late = 0;                                        // so far, in slot order
     auto place = [&](int r, const unsigned (&k)[4]) {
         const int s = r * ROUND + tid * 4;
