@@ -13,6 +13,7 @@
 // The rotated q is kept as three bf16 terms (24 bits) and p as two (15 bits): the products are then as good as float32 ones, and what is
 // rounded is what the caller asked to be rounded (stored keys, the output).  Each term but the last is truncated, so that all have one
 // sign, and none is 0 unless the value is: an infinite key or value gives what it gives in one product (inf - inf and 0 * inf do not arise).
+// A term that would be 0 beside one that is not is the least normal number, 2^-126, which is also where exp and the reciprocal end.
 // float32 runs the same walk on the f32 matrix instruction.
 // A workgroup is four waves that take 32 slots each in turn, with their own running maximum and sum, merged at the end; long caches
 // are split over workgroups and a second kernel joins them (and adds the weights up).  The token's own key and value are taken
@@ -209,7 +210,7 @@ template <typename T, int VE_, int NS_, int NT_, int AL, bool ST> struct Step {
         else {
             float least[PE];
 #pragma unroll
-            for (int e = 0; e < PE; e++) least[e] = x[e] == 0.f ? 0.f : copysignf(0x1p-100f, x[e]);
+            for (int e = 0; e < PE; e++) least[e] = x[e] == 0.f ? 0.f : copysignf(0x1p-126f, x[e]);
 #pragma unroll
             for (int t = 0; t < QT; t++) {
                 unsigned w[PE];
@@ -271,8 +272,9 @@ template <typename T, int VE_, int NS_, int NT_, int AL, bool ST> struct Step {
             for (int m = 0; m < W; m++) {
                 const unsigned a = __float_as_uint(p[2 * m]), b = __float_as_uint(p[2 * m + 1]);
                 hi[m] = __builtin_amdgcn_perm(b, a, 0x07060302u);
-                lo[m] = __builtin_bit_cast(unsigned, __builtin_convertvector((f2_t{fmaxf(p[2 * m] - __uint_as_float(a & 0xffff0000u), 0x1p-100f),
-                                                                                  fmaxf(p[2 * m + 1] - __uint_as_float(b & 0xffff0000u), 0x1p-100f)}), b2_t));
+                lo[m] = __builtin_bit_cast(unsigned, __builtin_convertvector(
+                    (f2_t{fmaxf(p[2 * m] - __uint_as_float(a & 0xffff0000u), fminf(p[2 * m], 0x1p-126f)),
+                          fmaxf(p[2 * m + 1] - __uint_as_float(b & 0xffff0000u), fminf(p[2 * m + 1], 0x1p-126f))}), b2_t));
             }
 #pragma unroll
             for (int e = 0; e < VE; e++) {

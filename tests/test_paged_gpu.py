@@ -296,6 +296,51 @@ def test_large_scores_do_not_overflow():
         _check_step(c, before, q, k, v, lens, 4, 0, (None, None), False, None, o)
 
 
+@pytest.mark.parametrize("stable", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_large_values_count_by_their_weight_alone(dtype, stable):
+    """Values of 2^100 in slots whose probability is nothing (softmax, 200 and more below the maximum: exp underflows) or about 2^-117
+    (stablemax's s(x) = 1 / (1 - x) far down): the sum gets p v of them and no more.  Each p may be off by 2^-126, the least normal number, on
+    top of the bound above, whose M is that of the ordinary slots: the others' p is relative to their score in stablemax, 0 in softmax."""
+    from multimodal_amd import ops
+    lens, H, d = [200, 1500], 2, 64
+    c, q, k, v = _filled(21, dtype, 2, 1, H, d, 16, lens)
+    q = (q.abs() + 0.5).to(dtype)
+    for b, n in enumerate(lens):
+        s = torch.arange(1, n, 3)
+        pg, off = c.table[b].cpu().long()[s // 16].to(DEV), (s % 16).to(DEV)
+        c.k[pg, :, off] = -(2.0 ** 112) if stable else -60.0
+        c.v[pg, :, off] = 2.0 ** 100
+    n_dev = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = ops.paged_decode_attn(q, None, None, c.k, c.v, c.table, n_dev, H, 0, None, None, stable).double().cpu()
+    for b, n in enumerate(lens):
+        Q, K, V = q[b].double().cpu().view(H, d), c.rows(c.k, b, n), c.rows(c.v, b, n)
+        there = torch.ones(n, dtype=torch.bool)
+        ordinary = there.clone(); ordinary[1::3] = False
+        want, _, p, _ = _attend(Q, K, V, there, stable, dtype)
+        E = _attend(Q, K, V, ordinary, stable, dtype)[3]
+        tol = HALF[dtype] * want.abs() + (E + (2.0 ** -15 if dtype == torch.bfloat16 else 0.0)) * (1 + 2.0 ** -7) * (p[..., None] * V.abs()).sum(1) \
+            + n * 2.0 ** -126 * 2.0 ** 100
+        assert ((o[b].view(H, d) - want).abs() <= tol).all(), (b, float((o[b].view(H, d) - want).abs().max()))
+
+
+def test_small_queries_of_large_keys():
+    """Rotated queries near 2^-100 of keys near 2^100: the scores are ordinary ones.  A term of q may be off by 2^-126, two of them a value."""
+    from multimodal_amd import ops
+    for dtype in (torch.bfloat16, torch.float32):
+        n, H, d = 90, 2, 64
+        c, q, _, _ = _filled(23, dtype, 1, 1, H, d, 16, [n])
+        q, c.k = (q.float() * 2.0 ** -100).to(dtype), (c.k.float() * 2.0 ** 100).to(dtype)
+        tabs = _tables(64, n)
+        o = ops.paged_decode_attn(q, None, None, c.k, c.v, c.table, torch.tensor([n], dtype=torch.int32, device=DEV), H, 64, *tabs, False).double().cpu()
+        Q, _ = _turn(q[0].double().cpu().view(H, d), tabs[0][n - 1].double().cpu(), tabs[1][n - 1].double().cpu(), 64)
+        K, V = c.rows(c.k, 0, n), c.rows(c.v, 0, n)
+        want, tol, p, _ = _attend(Q, K, V, torch.ones(n, dtype=torch.bool), False, dtype)
+        turned = 4 * U * float((K.abs() * 1.5 * Q.abs().max()).sum(-1).max()) / math.sqrt(d)          # rounding of the rotated q: as of stored keys
+        floor = 2 * 2.0 ** -126 * float(K.abs().sum(-1).max()) / math.sqrt(d)
+        assert ((o.view(H, d) - want).abs() <= tol + 2 * (turned + floor) * (p[..., None] * V.abs()).sum(1)).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_long_rows_beside_short_ones(dtype):
     """Lengths far apart in one call (the cache's length is split over workgroups), with weights."""
