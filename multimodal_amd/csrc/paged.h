@@ -20,6 +20,11 @@ static inline int paged_shift(int64_t page) {
     for (int s = 2; s <= 10; s++) if (page == (1 << s)) return s;
     return -1;
 }
+// whether what B rows' tables can name is more than the last-level cache (256 MB) holds: never more than the pool has, however wide the
+// tables are and however many rows share a page
+static inline bool paged_past_cache(int64_t B, int64_t Hkv, int64_t d, int64_t page, int64_t n_pages, int64_t width, int dtype) {
+    return (B * width < n_pages ? B * width : n_pages) > (256LL << 20) / (page * Hkv * d * (dtype == MM_BF16 ? 4 : 8));
+}
 // what every entry point asks of a pool and its table; 0 or a negative code with the message set
 static inline int paged_check(const char* who, const void* kpool, const void* vpool, const int* table, int64_t B, int64_t Hkv, int64_t d,
                               int64_t page, int64_t n_pages, int64_t width, int64_t ld_table, int dtype) {

@@ -734,8 +734,9 @@ extern "C" int mm_paged_decode_attn(const mm_paged_attn_args* a, void* stream) {
     // Four times q in LDS: not for more than four query heads a KV head unless the head is small.
     const bool lone = (p.G <= 4 || a->d <= 64) && r.nsplit == 1 && a->width * a->page <= 512 && blocks >= 2048;
     // A cache that the last-level cache (256 MB) cannot hold until the next call is read past it: 154 us for 164 at 849 MB; at 69 MB it
-    // would be 39 for 26.
-    const bool past = a->B * a->Hkv * a->width * a->page * a->d * (a->dtype == MM_BF16 ? 4 : 8) > (256LL << 20);
+    // would be 39 for 26.  It goes by the pool, not by rows and their width alone, as rows may share pages or be the same row: five tokens of
+    // each of 128 rows of 240 slots, 8 heads of 128, a pool of 126 MB: 73 us, 98 past the cache.
+    const bool past = paged_past_cache(a->B, a->Hkv, a->d, a->page, a->n_pages, a->width, a->dtype);
     const int64_t d = a->d;
     if (a->dtype == MM_F32) {
         if (d <= 64) paged_launch<float, 4, 1, 1, 2>(p, lone, past, st);

@@ -386,7 +386,7 @@ extern "C" size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page,
     return (size_t)(B * Hkv) * (size_t)(24 * room + (room ? 8 * recent : 0) + 16);
 }
 
-template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64_t cap, hipStream_t st) {
+template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64_t cap, bool past, hipStream_t st) {
     const dim3 grid((unsigned)B, (unsigned)p.map.Hkv);
     const int64_t heads = B * p.map.Hkv;
     // One workgroup does everything where there is little to move; else the moves and the shift spread over the card in launches of their
@@ -409,7 +409,7 @@ template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64
         const dim3 g(grid.x, grid.y, shifters + movers);
         // Where the rows' slots are more than the last-level cache holds, what is moved goes past it (384 heads halved from up to 8192 slots of 512
         // bytes: 170 us, 178 through it; 128 heads from 2000 to 1024, which it holds: 33 and 29).
-        if (heads * cap * p.units * (int64_t)sizeof(U) * 2 > (256LL << 20)) hipLaunchKernelGGL((evict_move_k<U, true>), g, dim3(MOVERS), 0, st, p, (int)shifters);
+        if (past) hipLaunchKernelGGL((evict_move_k<U, true>), g, dim3(MOVERS), 0, st, p, (int)shifters);
         else hipLaunchKernelGGL((evict_move_k<U, false>), g, dim3(MOVERS), 0, st, p, (int)shifters);
     }
     if (all) hipLaunchKernelGGL(evict_lengths_k, dim3(grid.x), dim3(64), 0, st, p);
@@ -434,9 +434,10 @@ extern "C" int mm_paged_evict(void* kpool, void* vpool, float* weights, const in
     p.kpool = (char*)kpool; p.vpool = (char*)vpool; p.w = weights; p.lengths = lengths; p.kept = kept;
     p.map = {page_table, (long)ld_table, (int)width, paged_shift(page), (int)n_pages, (int)Hkv};
     p.ws = (char*)workspace; p.room = (int)room; p.units = (int)(bytes / piece); p.budget = (int)budget; p.recent = (int)recent;
+    const bool past = paged_past_cache(B, Hkv, d, page, n_pages, width, dtype);
     hipStream_t st = (hipStream_t)stream;
-    if (piece == 16) evict_launch<mm_u4_t>(p, B, page * width, st);
-    else evict_launch<mm_u2_t>(p, B, page * width, st);
+    if (piece == 16) evict_launch<mm_u4_t>(p, B, page * width, past, st);
+    else evict_launch<mm_u2_t>(p, B, page * width, past, st);
     MM_LAUNCH_CHECK();
     return MM_OK;
 }

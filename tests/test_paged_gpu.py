@@ -387,6 +387,38 @@ def test_many_short_rows(dtype, G, d, width, weights):
         assert ((part.float() - o[s].float()).abs() <= 2 * HALF[dtype] * o[s].float().abs() + 2.0 ** -12 * float(o.float().abs().max())).all(), i
 
 
+@pytest.mark.parametrize("dtype,G,d", [(torch.bfloat16, 3, 128), (torch.float32, 1, 100), (torch.bfloat16, 8, 72), (torch.bfloat16, 1, 512), (torch.float32, 1, 512),
+                                       (torch.bfloat16, 5, 100), (torch.float32, 5, 200)])
+def test_pools_past_the_last_level_cache(dtype, G, d):
+    """Pools of more than 256 MB that the tables can name whole (read non-temporally), a wave a row and four: a few rows against the definition,
+    all of them against calls of a few rows, which read through the caches."""
+    from multimodal_amd import ops
+    B, Hkv, rot, width = 640, 4, d // 4 * 2, 32
+    g = torch.Generator().manual_seed(24)
+    lens = torch.randint(-1, 61, (B,), generator=g).tolist()
+    c, q, k, v = _filled(24, dtype, B, Hkv, G, d, 16, lens, spare=(256 << 20) // (16 * Hkv * d * 2 * dtype.itemsize) + 1)
+    c.table = torch.nn.functional.pad(c.table, (0, width - c.table.shape[1]), value=-1).contiguous()
+    assert min(c.n_pages, B * width) * 16 * Hkv * d * 2 * dtype.itemsize > 256 << 20
+    before = (c.k.clone(), c.v.clone(), None)
+    tabs = _tables(rot, 61)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    o = ops.paged_decode_attn(q, k, v, c.k, c.v, c.table, n, Hkv * G, rot, *tabs, False)
+    few = list(range(0, B, 53))
+    sub = Cache.__new__(Cache)
+    sub.__dict__.update(c.__dict__)
+    sub.table = c.table[few].contiguous()
+    mine = torch.zeros(c.n_pages, dtype=torch.bool, device=DEV)
+    mine[sub.table[sub.table >= 0].long()] = True
+    base = tuple(torch.where(mine.view(-1, 1, 1, 1), x, y) for x, y in zip(before, (c.k, c.v))) + (None,)
+    _check_step(sub, base, q[few], k[few], v[few], [lens[b] for b in few], Hkv * G, rot, tabs, False, None, o[few])
+    del before, base
+    for i in range(0, B, 64):
+        s = slice(i, i + 64)
+        part = ops.paged_decode_attn(q[s], None, None, c.k, c.v, c.table[s], torch.where(n[s] < 0, n[s], n[s] + 1), Hkv * G, rot, *tabs, False)
+        # as in test_many_short_rows
+        assert ((part.float() - o[s].float()).abs() <= 2 * HALF[dtype] * o[s].float().abs() + 2.0 ** -12 * float(o.float().abs().max())).all(), i
+
+
 def test_tables_far_wider_than_the_rows():
     """A table of 200000 slots for rows of a few: splits beyond a row's end do nothing."""
     from multimodal_amd import ops
@@ -725,6 +757,46 @@ def test_evict_many_slots_and_missing_pages():
                 x[pt, h, ot] = y[ps, h, os]
     for x, y in zip((c.k, c.v, c.w), want):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+def _evict_large(seed, dtype, B, Hkv, d, page, lens, budget, recent):
+    """An eviction of many slots: kept by a stable sort, the pools bit by bit, everything on the GPU.  Weights are distinct but for a tenth."""
+    from multimodal_amd import ops
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    width = -(-max(lens) // page)
+    n_pages = B * width + 3
+    table = torch.randperm(n_pages, generator=g, device=DEV)[: B * width].view(B, width)
+    k = torch.empty(n_pages, Hkv, page, d, dtype=dtype, device=DEV).normal_(generator=g)
+    v = torch.empty_like(k).normal_(generator=g)
+    w = torch.rand(n_pages, Hkv, page, generator=g, device=DEV)
+    w[w < 0.1] = 0.5
+    before = (k.clone(), v.clone(), w.clone())
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    kept = ops.paged_evict(k, v, w, table.int(), n, budget, recent)
+    assert n.tolist() == [min(x, budget) for x in lens]
+    A, j = budget - recent, torch.arange(budget, device=DEV)
+    hb = torch.arange(Hkv, device=DEV)[:, None]
+    for b, m in enumerate(lens):
+        if m <= budget:
+            assert (kept[b] == torch.where(j < m, j, -1)).all(), b
+            continue
+        ws = before[2][table[b]].transpose(0, 1).reshape(Hkv, -1)[:, : m - recent]
+        best = torch.zeros_like(ws, dtype=torch.bool).scatter_(1, ws.sort(dim=1, descending=True, stable=True).indices[:, :A], True)
+        want = torch.cat((j[:A].expand(Hkv, A), torch.arange(m - recent, m, device=DEV).expand(Hkv, recent)), 1).clone()
+        want[:, :A][~best[:, :A]] = best[:, A:].nonzero()[:, 1] + A                      # row by row, holes and survivors alike in order
+        assert torch.equal(kept[b].long(), want), b
+        for x, y in zip((k, v, w), before):
+            y[table[b][j // page][None], hb, (j % page)[None]] = y[table[b][want // page], hb, want % page].clone()
+    for x, y in zip((k, v, w), before):
+        assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float32, 100), (torch.bfloat16, 100)])
+def test_evict_past_the_last_level_cache(dtype, d):
+    """Pools of more than 256 MB: what moves goes past the cache (16- and 8-byte pieces)."""
+    lens = [4096, 4000, 2049, 2048, 1, 0] + [3000 + 37 * i for i in range(26)]
+    assert 32 * 8 * 4096 * d * 2 * dtype.itemsize > 256 << 20
+    _evict_large(45, dtype, 32, 8, d, 64, lens, 2048, 100)
 
 
 # ------------------------------------------------------------------------------------------------ together
