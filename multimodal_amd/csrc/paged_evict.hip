@@ -389,9 +389,11 @@ extern "C" size_t mm_paged_evict_workspace(int64_t B, int64_t Hkv, int64_t page,
 template <typename U> static void evict_launch(const EvictP& p, int64_t B, int64_t cap, bool past, hipStream_t st) {
     const dim3 grid((unsigned)B, (unsigned)p.map.Hkv);
     const int64_t heads = B * p.map.Hkv;
-    // One workgroup does everything where there is little to move; else the moves and the shift spread over the card in launches of their
-    // own (48 rows of up to 8192 slots and 8 KV heads, halved: 244 us in one launch, 170 in two).
-    const bool all = ((int64_t)p.room + p.recent) * p.units <= 8192;
+    // Rows and heads that fill the card with a workgroup each: one launch moves and shifts as well, where that is little (microseconds in one
+    // launch and in two: 768 heads cut from up to 300 slots of 256 bytes to 128 26 and 28, 1600 heads from 600 to 300 52 and 62, 9600 heads from
+    // 300 to 128 200 and 270).  Else the moves and the shift spread over the card in a launch of their own (32 heads from 300 to 128 17 and 15,
+    // 512 heads from 600 to 300 29 and 28, 128 heads from 1000 to 500 27 and 18, 384 heads from 8192 to 4096 217 and 170).
+    const bool all = heads >= 768 && ((int64_t)p.room + p.recent) * p.units <= 8192;
 #define MM_SELECT(NW_, R_) do { if (all) hipLaunchKernelGGL((evict_select_k<NW_, R_, U, true>), grid, dim3(NW_ * 64), 0, st, p); \
                                      else hipLaunchKernelGGL((evict_select_k<NW_, R_, U, false>), grid, dim3(NW_ * 64), 0, st, p); } while (0)
     if (cap <= 1024) MM_SELECT(4, 4);

@@ -759,34 +759,38 @@ def test_evict_many_slots_and_missing_pages():
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
 
-def _evict_large(seed, dtype, B, Hkv, d, page, lens, budget, recent):
-    """An eviction of many slots: kept by a stable sort, the pools bit by bit, everything on the GPU.  Weights are distinct but for a tenth."""
+def _evict_large(seed, dtype, B, Hkv, d, page, lens, budget, recent, missing=0.0):
+    """An eviction of many slots: kept by a stable sort, the pools bit by bit, everything on the GPU.  Weights are distinct but for a tenth;
+    missing: this share of the table's entries names no page."""
     from multimodal_amd import ops
     g = torch.Generator(device=DEV).manual_seed(seed)
     width = -(-max(lens) // page)
     n_pages = B * width + 3
     table = torch.randperm(n_pages, generator=g, device=DEV)[: B * width].view(B, width)
+    there = torch.rand(B, width, generator=g, device=DEV) >= missing
     k = torch.empty(n_pages, Hkv, page, d, dtype=dtype, device=DEV).normal_(generator=g)
     v = torch.empty_like(k).normal_(generator=g)
     w = torch.rand(n_pages, Hkv, page, generator=g, device=DEV)
     w[w < 0.1] = 0.5
     before = (k.clone(), v.clone(), w.clone())
     n = torch.tensor(lens, dtype=torch.int32, device=DEV)
-    kept = ops.paged_evict(k, v, w, table.int(), n, budget, recent)
+    kept = ops.paged_evict(k, v, w, torch.where(there, table, -1).int(), n, budget, recent)
     assert n.tolist() == [min(x, budget) for x in lens]
     A, j = budget - recent, torch.arange(budget, device=DEV)
-    hb = torch.arange(Hkv, device=DEV)[:, None]
     for b, m in enumerate(lens):
         if m <= budget:
             assert (kept[b] == torch.where(j < m, j, -1)).all(), b
             continue
-        ws = before[2][table[b]].transpose(0, 1).reshape(Hkv, -1)[:, : m - recent]
+        on = there[b].repeat_interleave(page)
+        ws = before[2][table[b]].transpose(0, 1).reshape(Hkv, -1).masked_fill(~on, -math.inf)[:, : m - recent]
         best = torch.zeros_like(ws, dtype=torch.bool).scatter_(1, ws.sort(dim=1, descending=True, stable=True).indices[:, :A], True)
         want = torch.cat((j[:A].expand(Hkv, A), torch.arange(m - recent, m, device=DEV).expand(Hkv, recent)), 1).clone()
         want[:, :A][~best[:, :A]] = best[:, A:].nonzero()[:, 1] + A                      # row by row, holes and survivors alike in order
         assert torch.equal(kept[b].long(), want), b
-        for x, y in zip((k, v, w), before):
-            y[table[b][j // page][None], hb, (j % page)[None]] = y[table[b][want // page], hb, want % page].clone()
+        h, to = (on[want] & on[j]).nonzero(as_tuple=True)
+        src = want[h, to]
+        for y in before:
+            y[table[b][to // page], h, to % page] = y[table[b][src // page], h, src % page].clone()
     for x, y in zip((k, v, w), before):
         assert torch.equal(x.view(torch.uint8), y.view(torch.uint8))
 
@@ -797,6 +801,18 @@ def test_evict_past_the_last_level_cache(dtype, d):
     lens = [4096, 4000, 2049, 2048, 1, 0] + [3000 + 37 * i for i in range(26)]
     assert 32 * 8 * 4096 * d * 2 * dtype.itemsize > 256 << 20
     _evict_large(45, dtype, 32, 8, d, 64, lens, 2048, 100)
+
+
+@pytest.mark.parametrize("dtype,Hkv,d,page,longest,budget,recent", [
+    (torch.bfloat16, 8, 64, 16, 300, 64, 16), (torch.float32, 2, 100, 16, 200, 40, 0), (torch.bfloat16, 8, 128, 8, 90, 33, 33),
+    (torch.bfloat16, 4, 36, 16, 2000, 100, 20), (torch.bfloat16, 1, 8, 1024, 12000, 60, 5), (torch.bfloat16, 1, 4, 1024, 40000, 300, 30),
+    (torch.bfloat16, 1, 4, 1024, 70000, 300, 30)])
+def test_evict_many_rows(dtype, Hkv, d, page, longest, budget, recent):
+    """Rows and heads that fill the card, of every length: a workgroup each does it all."""
+    B = 800 // min(Hkv, 4) + 7
+    lens = [1 + (longest - 1) * i // (B - 1) for i in range(B)]
+    _evict_large(46, dtype, B, Hkv, d, page, lens[::-1], budget, recent)
+    _evict_large(47, dtype, B, Hkv, d, page, lens, budget, recent, missing=0.1)
 
 
 # ------------------------------------------------------------------------------------------------ together
