@@ -50,7 +50,7 @@ class PagedKVCache:
         for k, v, w in zip(self.k, self.v, self.w):
             n = self.lengths.clone()
             ops.paged_evict(k, v, w, self.page_table, n, budget, recent)
-        self.lengths = n
+        self.lengths.copy_(n)                          # in place: who holds the tensor (a captured step among them) reads it
 
 
 def _layer_weights(layer, dt):

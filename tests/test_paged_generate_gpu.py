@@ -77,6 +77,18 @@ def test_budget_bounds_the_cache_and_keeps_what_comes_before_the_first_eviction(
     assert ((got >= 0) & (got < 591)).all()
 
 
+def test_eviction_writes_the_lengths_in_place():
+    """Lengths held from before (a captured step reads them where they were) say what the rows hold after it; every layer is cut alike."""
+    from multimodal_amd.generate import PagedKVCache
+    c = PagedKVCache(3, 4, 2, 64, 32, 16, torch.float32, DEV, weights=True)
+    for t in c.k + c.v + c.w:
+        t.normal_()
+    mine = c.lengths
+    mine.copy_(torch.tensor([50, 20, 0, 33], device=DEV))
+    c.evict(24, 8)
+    assert c.lengths is mine and mine.tolist() == [24, 20, 0, 24]
+
+
 def test_budget_arguments():
     m = _model(3)
     nmr, ir = _inputs(2)
