@@ -340,8 +340,9 @@ def speculative_generate(model, draft, nmr_tokens: Optional[torch.Tensor], ir_da
     distributed as the model's own samples at this temperature.  Rows accept different numbers of tokens, so their caches are paged.
     temperature=0: greedy, the ids of generate() up to each row's end (near-ties aside: the passes are of other shapes).  Returns int64
     [B, <= max_len+1]: BOS, the tokens up to EOS or max_len of them, then pad_id."""
-    if n_draft < 1 or temperature < 0:
-        raise ValueError(f"speculative_generate: n_draft={n_draft} (at least 1), temperature={temperature} (not negative)")
+    if n_draft < 1 or page_size <= 0 or not (temperature == 0 or temperature >= 1e-30):        # logits / temperature stay finite
+        raise ValueError(f"speculative_generate: n_draft={n_draft} (at least 1), page_size={page_size} (a power of two, 4 to 1024), "
+                         f"temperature={temperature} (0 or at least 1e-30)")
     if model.decoder.out.weight.shape[0] != draft.decoder.out.weight.shape[0]:
         raise ValueError("speculative_generate: model and draft must share one vocabulary")
     FN.flush_deferred_updates()
@@ -421,10 +422,13 @@ def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Te
     if page_size is not None or kv_budget is not None:
         if graph:
             raise ValueError("greedy_generate: graph=True runs on the dense cache only")
+        if page_size is not None and page_size <= 0:
+            raise ValueError(f"greedy_generate: page_size={page_size} (a power of two, 4 to 1024)")
         if kv_budget is not None and not 0 < kv_recent <= kv_budget:
             raise ValueError(f"greedy_generate: kv_recent={kv_recent} must be between 1 and kv_budget={kv_budget}")
         try:
-            return _paged_greedy(model, nmr_tokens, ir_data, max_len, bos_id, eos_id, early_stop, sync_every, page_size or 16, kv_budget, kv_recent)
+            return _paged_greedy(model, nmr_tokens, ir_data, max_len, bos_id, eos_id, early_stop, sync_every, 16 if page_size is None else page_size,
+                                 kv_budget, kv_recent)
         finally:
             model.train(was_training)
     dev = ir_data.device

@@ -169,3 +169,19 @@ def test_drafting_refuses():
     for kw in (dict(n_draft=0), dict(temperature=-1.0)):
         with pytest.raises(ValueError):
             speculative_generate(m, m, nmr, ir, **kw)
+
+
+def test_sizes_and_temperatures_that_mean_nothing_are_refused():
+    """page_size=0 is not the default's 16; a temperature that is no number, or so small that logits divided by it are infinite, has no softmax."""
+    from multimodal_amd.generate import speculative_generate
+    m = _model(9)
+    nmr, ir = _inputs(2)
+    for kw in (dict(page_size=0), dict(page_size=-16), dict(page_size=0, kv_budget=20)):
+        with pytest.raises(ValueError, match="page_size"):
+            m.generate(nmr, ir, max_len=4, **kw)
+    for kw in (dict(temperature=float("nan")), dict(temperature=1e-39), dict(page_size=0)):
+        with pytest.raises(ValueError):
+            speculative_generate(m, m, nmr, ir, max_len=4, **kw)
+    # the smallest one is the greedy choice
+    a = speculative_generate(m, m, nmr, ir, max_len=6, n_draft=2, temperature=1e-30, eos_id=-7)
+    assert torch.equal(a, m.generate(nmr, ir, max_len=6, early_stop=False))
