@@ -72,6 +72,44 @@ def test_against_the_definition(shape, with_q):
     _check(x, p, u, q if with_q else None, counts)
 
 
+@pytest.mark.parametrize("with_q", [True, False])
+@pytest.mark.parametrize("shape", [(130, 2, 50000), (128, 1, 12545), (1, 2, 1048577 + 300), (2, 1, 3000001)], ids=str)
+def test_large_vocabularies(shape, with_q):
+    """A workgroup a row with several blocks in flight (128 rows and more); blocks of more than 256 values (past 2^20), rows split over workgroups."""
+    x, p, u, q, g = _inputs(11, *shape)
+    _check(x, p, u, q if with_q else None)
+    counts = torch.randint(0, shape[1] + 1, (shape[0],), generator=g).int().to(DEV)
+    _check(x, p, u, q if with_q else None, counts)
+
+
+def test_many_rows_of_a_vocabulary_past_2_to_the_20():
+    """One distribution (batch stride 0), 200 random numbers: the place in its cumulative sum."""
+    from multimodal_amd import ops
+    V, B = 1048576 + 4099, 200
+    g = torch.Generator().manual_seed(12)
+    p = torch.softmax(torch.randn(V, generator=g) * 2, 0)
+    u = torch.rand(B, 1, generator=g)
+    c = p.double().numpy().cumsum()
+    t = u[:, 0].double().numpy() * c[-1]
+    want = np.searchsorted(c, t, side="right")
+    assert (np.abs(c[want] - t) > 2.0 ** -40).all() and (np.abs(c[np.maximum(want - 1, 0)] - t) > 2.0 ** -40).all(), "input on a border"
+    got, acc = ops.verify_drafts(torch.zeros(B, 0, dtype=torch.long, device=DEV), p.to(DEV).expand(B, 1, V), u.to(DEV))
+    assert (got[:, 0].cpu().numpy() == want).all() and (acc == 0).all()
+
+
+@pytest.mark.parametrize("B", [2, 130])
+def test_empty_residuals_of_large_vocabularies(B):
+    """p is half of q everywhere and the draft is rejected: nothing is left of p - q, so the last token is drawn from p itself.  Every third row's
+    p is q: its draft is accepted."""
+    _, p, u, q, g = _inputs(13, B, 1, 50000)
+    p = torch.cat((q * 0.5, p[:, 1:]), 1)
+    p[2::3, 0] = q[2::3, 0]
+    x = torch.randint(0, 50000, (B, 1), generator=g).to(DEV)
+    u[:, 0] = 0.5 + 0.25 * u[:, 0]
+    acc = _check(x, p.contiguous(), u, q)
+    assert acc.tolist() == [1 if b % 3 == 2 else 0 for b in range(B)]
+
+
 def test_every_number_of_accepted_drafts_occurs():
     x, p, u, q, _ = _inputs(2, 400, 4, 50)
     acc = _check(x, p, u, q)
