@@ -12,7 +12,7 @@
 //     transposes 8 x 8 values in registers (32 v_perm per 128 columns), which is the A operand.  No LDS traffic in the loop.
 // The rotated q is kept as three bf16 terms (24 bits) and p as two (15 bits): the products are then as good as float32 ones, and what is
 // rounded is what the caller asked to be rounded (stored keys, the output).  Each term but the last is truncated, so that all have one
-// sign, and none is 0 unless the value is: an infinite key or value gives what it gives in one product (inf - inf and 0 * inf do not arise).
+// sign, and none is 0 unless the value is: an infinite query, key or value gives what it gives in one product (inf - inf and 0 * inf do not arise).
 // A term that would be 0 beside one that is not is the least normal number, 2^-126, which is also where exp and the reciprocal end.
 // float32 runs the same walk on the f32 matrix instruction.
 // A workgroup is four waves that take 32 slots each in turn, with their own running maximum and sum, merged at the end; long caches
@@ -218,7 +218,7 @@ template <typename T, int VE_, int NS_, int NT_, int AL, bool ST> struct Step {
                 for (int e = 0; e < PE; e++) {
                     const float h = __uint_as_float(__float_as_uint(x[e]) & 0xffff0000u);
                     w[e] = __float_as_uint(t && h == 0.f ? least[e] : h);
-                    x[e] -= h;
+                    x[e] = x[e] == h ? 0.f : x[e] - h;                             // inf leaves nothing
                 }
                 *reinterpret_cast<u4_t*>(f + t * heads * QS) =
                     u4_t{w[0] >> 16 | w[1], w[2] >> 16 | w[3], w[4] >> 16 | w[5], w[6] >> 16 | w[7]};

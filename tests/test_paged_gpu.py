@@ -284,6 +284,24 @@ def test_an_infinite_key_weighs_nothing_or_everything():
             assert ((o.double().cpu().view(1, 64) - want).abs() <= tol).all()
 
 
+def test_an_infinite_query_weighs_its_keys_by_sign():
+    """A rotated query with an infinite pair: keys that are negative there score -inf.  Where all are, the row is without weight; where the others
+    are 0 there, or positive, there is no finite answer."""
+    from multimodal_amd import ops
+    for dtype in (torch.bfloat16, torch.float32):
+        for stable in (False, True):
+            c, q, k, v = _filled(25, dtype, 2, 1, 2, 64, 16, [50, 50])
+            q = q.clone()
+            q[:, 7], q[:, 39] = math.inf, 1.0                                             # the pair (7, 39) of head 0; head 1 is finite
+            c.k[..., 7], c.k[..., 39] = -0.5, -0.25
+            c.k[int(c.table[1, 1]), 0, 3, 7] = 0.5
+            c.k[int(c.table[1, 1]), 0, 3, 39] = 0.5
+            tabs = tuple(torch.full((50, 32), x, device=DEV) for x in (0.8, 0.6))         # both of the pair become +inf
+            n = torch.tensor([50, 50], dtype=torch.int32, device=DEV)
+            o = ops.paged_decode_attn(q, None, None, c.k, c.v, c.table, n, 2, 64, *tabs, stable).float().view(2, 2, 64)
+            assert (o[0, 0] == 0).all() and torch.isnan(o[1, 0]).all() and torch.isfinite(o[:, 1]).all(), (dtype, stable)
+
+
 def test_large_scores_do_not_overflow():
     """Scores far beyond exp's range, of both signs: the running maximum keeps the sums finite."""
     from multimodal_amd import ops
