@@ -404,10 +404,12 @@ def speculative_generate(model, draft, nmr_tokens: Optional[torch.Tensor], ir_da
 def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Tensor, max_len: int = 128, bos_id: int = 12,
                     eos_id: int = 13, early_stop: bool = True, sync_every: int = 8, graph: Optional[bool] = None,
                     page_size: Optional[int] = None, kv_budget: Optional[int] = None, kv_recent: int = 16) -> torch.Tensor:
-    """page_size: keep the keys and values in pages of so many slots (PagedKVCache) instead of one dense array per layer.  kv_budget: keep at
-    most so many slots of a row between evictions (page_size defaults to 16): every kv_recent tokens each layer's heads drop the older
-    slots that have drawn the least attention, and the kv_recent newest always stay; memory per row is then bounded, and the ids are
-    those of the pruned attention.
+    """page_size: keep the keys and values in pages of so many slots (PagedKVCache) instead of one dense array per layer.  kv_budget: cut
+    every row down to so many slots again and again (page_size defaults to 16): every kv_recent tokens each layer's heads drop the older
+    slots that have drawn the least attention, and the kv_recent newest always stay.  A row holds up to kv_budget + kv_recent slots between
+    two evictions, and before the first one its whole prompt and kv_recent tokens: max(kv_budget, prompt) + kv_recent slots are what the
+    cache is made for.  The ids are those of the pruned attention.  What counts is the attention drawn by the tokens behind the prompt: the
+    prompt's own pass leaves no weights, so the first eviction goes by kv_recent rows of attention.
 
     graph=True: replay the decode step from ONE captured HIP graph (position, output column and current ids live in device
     memory and advance inside the graph).  Same kernels, same ids as the eager loop (tested), but OFF by default: on this

@@ -464,7 +464,9 @@ def paged_decode_attn(q: Tensor, k_new: Optional[Tensor], v_new: Optional[Tensor
     attends over slots 0 .. lengths[b]; the caller advances lengths.  k_new = v_new = None: q attends over the stored slots alone (rows
     of drafted tokens stored by paged_cache_fill: one row per token, the table's row repeated).  positions int32 [B]: the rotary
     position where it is not the slot (after paged_evict).  weights float32 [pages, Hkv, page]: accumulates the attention each slot
-    draws (paged_evict goes by it).  A row with lengths < 0 sits out; a row without a slot, and one that sits out, gets zeros.  A token
+    draws (paged_evict goes by it).  The launch, and with weights the workspace (B * H floats a slot), are laid out for the table's width:
+    pass table[:, :pages the longest row needs] where it is known (1024 rows of 160 to 300 slots under tables of 32768 slots: 365 us, 173 under
+    table[:, :19]).  A row with lengths < 0 sits out; a row without a slot, and one that sits out, gets zeros.  A token
     whose page the table does not hold is neither stored nor attended.  Pages written by a call belong to one row, with weights all that
     it attends over.  Returns o [B, H*d]."""
     who = "paged_decode_attn"
