@@ -416,18 +416,19 @@ def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Te
     stack (ROCm 7.2) replaying the ~45-node step costs more than issuing it -- nocat shape, 80 steps: B=1024 549k vs 643k
     tokens/s eager, B=128 181k vs 178k -- the decode loop is not host-bound (unlike the small-config train step, where
     graph.CapturedTrainStep pays)."""
+    paged = page_size is not None or kv_budget is not None
+    if paged and graph:
+        raise ValueError("greedy_generate: graph=True runs on the dense cache only")
+    if page_size is not None and page_size <= 0:
+        raise ValueError(f"greedy_generate: page_size={page_size} (a power of two, 4 to 1024)")
+    if kv_budget is not None and not 0 < kv_recent <= kv_budget:
+        raise ValueError(f"greedy_generate: kv_recent={kv_recent} must be between 1 and kv_budget={kv_budget}")
     dec = model.decoder
     dt = FN.get_compute_dtype()
     FN.flush_deferred_updates()        # this loop reads the weights directly, not through model.forward (optim: deferred updates)
     was_training = model.training
     model.eval()
-    if page_size is not None or kv_budget is not None:
-        if graph:
-            raise ValueError("greedy_generate: graph=True runs on the dense cache only")
-        if page_size is not None and page_size <= 0:
-            raise ValueError(f"greedy_generate: page_size={page_size} (a power of two, 4 to 1024)")
-        if kv_budget is not None and not 0 < kv_recent <= kv_budget:
-            raise ValueError(f"greedy_generate: kv_recent={kv_recent} must be between 1 and kv_budget={kv_budget}")
+    if paged:
         try:
             return _paged_greedy(model, nmr_tokens, ir_data, max_len, bos_id, eos_id, early_stop, sync_every, 16 if page_size is None else page_size,
                                  kv_budget, kv_recent)

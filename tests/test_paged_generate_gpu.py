@@ -185,3 +185,14 @@ def test_sizes_and_temperatures_that_mean_nothing_are_refused():
     # the smallest one is the greedy choice
     a = speculative_generate(m, m, nmr, ir, max_len=6, n_draft=2, temperature=1e-30, eos_id=-7)
     assert torch.equal(a, m.generate(nmr, ir, max_len=6, early_stop=False))
+
+
+def test_a_refused_call_leaves_the_model_in_training_mode():
+    m = _model(9)
+    nmr, ir = _inputs(2)
+    m.train()
+    for kw, kind in ((dict(page_size=0), ValueError), (dict(page_size=16, graph=True), ValueError), (dict(kv_budget=8, kv_recent=9), ValueError),
+                     (dict(page_size=12), RuntimeError)):
+        with pytest.raises(kind):
+            m.generate(nmr, ir, max_len=4, **kw)
+        assert m.training and m.decoder.training, kw
