@@ -346,9 +346,10 @@ __global__ __launch_bounds__(256) void dwconv7_ln_fwd_bcl(const T* __restrict__ 
 // ------------------------------------------------------------------------------------------------
 // The arithmetic is written on explicit pairs of channels (f2_t), two scalar instructions a pair: packed float32 instructions are off in
 // every source (Makefile).  With them these kernels were faster in bf16: 189 / 194 / 207 us for 198 / 203 / 217 in the strip kernel (C 64 /
-// 128 / 256, batch 8192), 277 / 299 for 308 / 331 in the wide one (C 1600 / 2048, batch 2048); float32 is the same either way.  Left to the SLP vectoriser the same loop held 126 v_mov_b32 per 8 rows that only
-// assembled pairs it had chosen across taps, and 80 selects for the zero padding (now done on the packed row before unpacking).
-// Registers: 186 (bf16) / 229 (f32) VGPRs, two waves per SIMD.  A cap at 168 or 128 (three / four waves) makes the compiler spill
+// 128 / 256, batch 8192), 277 / 299 for 308 / 331 in the wide one (C 1600 / 2048, batch 2048); float32 is the same either way.  Left to the SLP
+// vectoriser the same loop held 126 v_mov_b32 per 8 rows that only assembled pairs it had chosen across taps, and 80 selects for the
+// zero padding (now done on the packed row before unpacking).
+// Registers: 180-188 (bf16) / 216-233 (f32) VGPRs, two waves per SIMD.  A cap at 168 or 128 (three / four waves) makes the compiler spill
 // the rings to scratch inside the loop: 420 us (bf16) and 1570 us (f32) against 231 / 339 at B8192 C64 L250.
 typedef float f2_t __attribute__((ext_vector_type(2)));
 static __device__ __forceinline__ f2_t fma2(f2_t a, f2_t b, f2_t c) { return __builtin_elementwise_fma(a, b, c); }

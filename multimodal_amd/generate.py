@@ -409,7 +409,7 @@ def greedy_generate(model, nmr_tokens: Optional[torch.Tensor], ir_data: torch.Te
     slots that have drawn the least attention, and the kv_recent newest always stay.  A row holds up to kv_budget + kv_recent slots between
     two evictions, and before the first one its whole prompt and kv_recent tokens: max(kv_budget, prompt) + kv_recent slots are what the
     cache is made for.  The ids are those of the pruned attention.  What counts is the attention drawn by the tokens behind the prompt: the
-    prompt's own pass leaves no weights, so the first eviction goes by kv_recent rows of attention.
+    prompt's own pass leaves no weights, so that of a prompt longer than the budget kv_recent rows of attention decide.
 
     graph=True: replay the decode step from ONE captured HIP graph (position, output column and current ids live in device
     memory and advance inside the graph).  Same kernels, same ids as the eager loop (tested), but OFF by default: on this
